@@ -29,11 +29,10 @@ __device__ __forceinline__ float gelu_tanh_f(float x) {
     const float u = 0.79788456080286535588f * x * (1.0f + 0.044715f * x * x);
     return x * __builtin_amdgcn_rcpf(1.0f + __expf(-2.0f * u));
 }
-// The same GELU for the four accumulator values a lane owns, written on float2 so that hipcc emits packed-f32 VALU (v_pk_mul_f32 / v_pk_fma_f32 /
-// v_pk_add_f32: two elements per full-rate instruction) and with the constants folded: per PAIR 1 add (bias, done by the caller) + 3 mul + 1 fma
-// + 1 add packed, 2 v_exp_f32 + 2 v_rcp_f32, and -- ROUND_IN, ggml's f16 GELU table input -- one v_cvt_pk_f16_f32 (RNE) + two v_cvt_f32_f16.
-// The scalar form above compiled to 6 v_mul + 2 v_add + 1 v_fma + 1 v_cndmask per ELEMENT beside the two transcendentals (r04: FC1 epilogue
-// ISA), i.e. ~76 issue cycles per element against ~52 here.  exp(-2u) = 2^(x * (C1 + C3 x^2)), C1 = -2 sqrt(2/pi) log2(e), C3 = 0.044715 C1.
+// The same GELU for the four accumulator values a lane owns, two at a time with the constants folded: per element 1 add (bias, done by the caller) +
+// 3 mul + 1 fma + 1 add, 1 v_exp_f32 + 1 v_rcp_f32, and -- ROUND_IN, ggml's f16 GELU table input -- half a v_cvt_pk_f16_f32 (RNE) + one v_cvt_f32_f16.
+// (The build forbids packed-f32 instructions, build.py; with them the large-v3 benchmark ran no faster: 3201 / 3257 against 3307 / 3282 xRT, two runs
+// of each in turn.)  exp(-2u) = 2^(x * (C1 + C3 x^2)), C1 = -2 sqrt(2/pi) log2(e), C3 = 0.044715 C1.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 template <bool ROUND_IN>
