@@ -353,6 +353,106 @@ int ss_engine_selftest_gemm_ex(ss_engine* e, int32_t M, int32_t N, int32_t K, in
  * quantises its weights with at load (w / scale_n, scale_n = amax_n / 448), identical to gfx950's v_cvt_pk_fp8_f32. */
 int ss_e4m3_from_f32(const float* x, uint8_t* codes, int64_t n);
 
+/* ---- decoder operators on the caller's device buffers ------------------------------------------------
+ * For a program that keeps its own decoding loop beside the engine: a paged key / value cache in 16 or 8 bits, attention over it, and a sampler
+ * for the logits (the engine's own ss_process_logits picks the best id; ss_sample_rows draws).  They need no engine and no model.
+ *
+ * All pointers are device memory of `device` unless said otherwise; `stream` is a hipStream_t (NULL = the default stream).  A call checks its
+ * arguments (SS_ERR_ARG with the reason in ss_last_error), launches on `stream` and returns; it allocates nothing, keeps nothing between calls, never
+ * waits for the GPU and leaves the calling thread's current device as it was, so it may be captured into a graph.  Structs are read during the call
+ * only.  What lies in device memory cannot be checked on the host: the kernels check every page number, span and length before they use it
+ * (described at each call), and never read or write outside the buffers that the structs describe.
+ *
+ * Two calls may run at the same time if neither writes what the other uses; the workspace of ss_kv_attention counts as written. */
+enum { SS_DTYPE_F32 = 3 };                                      /* ss_sample_rows' logits only; no engine computes in it */
+enum { SS_KV_SAME = 0, SS_KV_E4M3 = 1, SS_KV_INT8 = 2 };
+typedef struct ss_kv_cache {      /* one layer */
+    void* k;                      /* [n_pages][n_kv_heads][page_size][head_dim] codes, a page contiguous; 16-byte aligned */
+    void* v;
+    void* k_scale;                /* [n_pages][n_kv_heads][page_size], NULL for SS_KV_SAME: */
+    void* v_scale;                /*   SS_KV_E4M3 uint8 E8M0 exponents, SS_KV_INT8 float32; 16-byte aligned */
+    int64_t page_stride;          /* elements from one page of k (and v) to the next: >= n_kv_heads * page_size * head_dim, a multiple of 16 */
+    int64_t scale_stride;         /* elements from one page of the scales to the next: >= n_kv_heads * page_size, a multiple of 16 */
+    int32_t n_pages;
+    int32_t page_size;            /* a power of two from 16 to 256 */
+    int32_t n_kv_heads;
+    int32_t head_dim;             /* 64 or 128 */
+    int32_t dtype;                /* SS_DTYPE_F16 or SS_DTYPE_BF16: the tokens' side (new keys and values, queries, results) */
+    int32_t kind;                 /* SS_KV_SAME: the cache holds dtype.
+                                     SS_KV_E4M3: OCP e4m3 codes with one power-of-two scale per (page, head, row), value = code * 2^(exponent - 127), the
+                                       least exponent with amax / 2^(exponent - 127) <= 448, codes rounded to nearest even (the fp8 engine's cross cache).
+                                     SS_KV_INT8: codes -127..127 = rint(x / scale), scale = amax / 127 in float32; a row of zeros has scale 0 */
+} ss_kv_cache;
+typedef struct ss_kv_batch {      /* the sequences of one step */
+    const int32_t* page_table;    /* [n_seqs] rows of max_pages entries: position p of the sequence lies in row p % page_size of page entry[p / page_size].
+                                     An entry outside [0, n_pages) (-1 for "none") holds nothing */
+    const int32_t* q_start;       /* [n_seqs + 1], non-decreasing: sequence s owns token rows [q_start[s], q_start[s + 1]); a span that decreases or
+                                     leaves [0, n_tokens] counts as empty.  Token rows that no sequence owns are neither read nor written */
+    const int32_t* kv_len;        /* [n_seqs] positions held, the new ones among them: new token i of n sits at position kv_len - n + i.  Positions below 0
+                                     or behind max_pages * page_size do not exist */
+    int64_t table_stride;         /* elements between rows of page_table, >= max_pages */
+    int32_t n_seqs;
+    int32_t max_pages;            /* max_pages * page_size < 2^30 */
+    int32_t n_tokens;             /* rows of the token tensors */
+    int32_t max_new;              /* at least the longest span (what a scheduler knows on the host): ss_kv_attention covers max_new tokens per sequence */
+    int32_t min_new;              /* the shortest span, or 0 if unknown: a hint that can save a launch */
+    int32_t max_len;              /* about the longest kv_len, or 0 if unknown: decides only how the keys are cut over workgroups */
+} ss_kv_batch;
+typedef struct ss_kv_rows {       /* [n_tokens][heads][head_dim] of dtype: 16-byte aligned, the head's elements contiguous */
+    void* p;
+    int64_t row_stride;           /* elements, multiples of 8; for results the rows must not overlap */
+    int64_t head_stride;
+} ss_kv_rows;
+int32_t ss_sizeof_kv_cache(void);
+int32_t ss_sizeof_kv_batch(void);
+int32_t ss_sizeof_kv_rows(void);
+/* Writes the new tokens' keys and values [n_tokens][n_kv_heads][head_dim] into their pages, in the cache's form.  Tokens whose position does not exist
+ * or lies on no page are dropped.  No two tokens of a call may share a position of a page (the program copies a shared page before it
+ * writes to it).  A row that holds a NaN or an infinity reads back as such, and in an 8-bit cache it may take the rest of its row with it. */
+int ss_kv_append(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_rows* k, const ss_kv_rows* v, int32_t device, void* stream);
+/* The reverse: fills k and v [n_tokens][n_kv_heads][head_dim] with what the cache holds at the tokens' positions, code * scale in float32 rounded once to
+ * dtype.  A whole context is read as kv_len tokens.  Positions that do not exist or lie on no page read as zeros. */
+int ss_kv_read(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_rows* k, const ss_kv_rows* v, int32_t device, void* stream);
+/* softmax(scale q K^T) V of the new tokens' queries [n_tokens][n_heads][head_dim] over their sequence's keys, which ss_kv_append has written, the new
+ * ones among them.  Query head i reads key head i / (n_heads / n_kv_heads).  causal != 0: a token sees the positions up to its own; 0: all kv_len of
+ * them (cross-attention).  Keys on no page are not seen.  A token that sees no key gets zeros (lse -inf).  Rows of pages behind kv_len may hold anything; keys
+ * and values that some token of the sequence sees are taken to be finite.
+ * out: as q.  lse (optional): float32 [n_tokens][n_heads], the natural logarithm of the softmax's denominator, with which results over disjoint keys
+ * are joined.  Softmax and sums are held in float32; the probabilities are rounded to the type that the matrix product takes (dtype; f16 for 8-bit
+ * caches, whose codes it holds exactly).  Results do not depend on the run, but the order of their sums does on max_new, min_new, max_len and n_seqs.
+ * workspace: ss_kv_attention_workspace(...) bytes, 16-byte aligned, NULL if that is 0; contents before and after mean nothing. */
+int64_t ss_kv_attention_workspace(const ss_kv_cache* cache, const ss_kv_batch* batch, int32_t n_heads);   /* < 0: SS_ERR_ARG.  Host only */
+int ss_kv_attention(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_rows* q, int32_t n_heads, float scale, int32_t causal, const ss_kv_rows* out,
+                    float* lse, void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
+
+/* Draws one id per row of logits.  With x the row (NaN counts as -inf, "masked") and t its temperature, w_i = exp((x_i - max x) / t); ids at +inf share all
+ * weight.  The filters, in this order: top_k keeps the k largest logits (ties: the lowest ids); top_p keeps an id while those before it, in order of
+ * weight (ties: of id), have less than top_p of what top_k left; min_p keeps ids with w_i >= min_p.  The best id is always kept.  Drawn is the first kept id, in
+ * order of id, whose running sum of kept weights exceeds u times their total: std::discrete_distribution's rule for a given uniform number.
+ * Weights are held as integers of 2^-bits of the largest (bits = 62 - log2 of the vocabulary, rounded down), so sums are exact and
+ * do not depend on the order; a draw can differ from the real numbers' only where u falls within about 1e-12 of a boundary.
+ * Settings per row may be NULL (off; temperature 1) and need no host value: t <= 0 or NaN takes the best id, top_k <= 0 or >= n_vocab, top_p >= 1 or NaN, min_p <= 0
+ * or NaN switch a filter off; u is taken into [0, 1).  A row without any unmasked id gives id -1, p 0, logprob -inf, n_kept 0. */
+typedef struct ss_sample_rows_args {
+    const void* logits;           /* [n_rows] rows of n_vocab, dtype, aligned to its size */
+    const double* u;              /* [n_rows] uniform numbers; the engine's generator gives doubles too */
+    const float* temperature;     /* [n_rows] each */
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int32_t* id;                  /* [n_rows] results */
+    float* p;                     /* weight of the id among the kept ones (1 where t <= 0); may be NULL */
+    float* logprob;               /* ln of its probability before the filters, at temperature t (1 where t <= 0); may be NULL */
+    int32_t* n_kept;              /* ids left by the filters (1 where t <= 0); may be NULL */
+    int64_t row_stride;           /* elements, >= n_vocab */
+    int32_t n_rows;
+    int32_t n_vocab;              /* <= 2^20 */
+    int32_t dtype;                /* SS_DTYPE_F32, SS_DTYPE_F16 or SS_DTYPE_BF16 */
+    int32_t reserved;
+} ss_sample_rows_args;
+int32_t ss_sizeof_sample_rows_args(void);
+int ss_sample_rows(const ss_sample_rows_args* args, int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,6 +4,7 @@
 #include <unordered_set>
 
 #include "engine.h"
+#include "ops.h"
 
 using namespace ss;
 
@@ -526,6 +527,158 @@ int ss_engine_selftest_gemm_ex(ss_engine* e, int32_t M, int32_t N, int32_t K, in
 int ss_engine_probe_gemm(ss_engine* e, int32_t batch, int32_t reps, float* avg_ms, double* flops) {
     if (!e || !avg_ms || !flops || reps <= 0) return fail(SS_ERR_ARG, "bad argument");
     SS_TRY e->e->probe_gemm(batch, reps, avg_ms, flops); return SS_OK; SS_CATCH
+}
+
+// ---- decoder operators on the caller's device buffers ----
+}  // extern "C"
+
+namespace {
+struct OnDevice {            // the caller's device for the time of a call; the thread's current one afterwards
+    int before = 0;
+    bool moved = false;
+    explicit OnDevice(int device) {
+        SS_HIP(hipGetDevice(&before));
+        if (device == before) return;
+        int n = 0;
+        SS_HIP(hipGetDeviceCount(&n));      // asked first: a failing hipSetDevice leaves an error that the next launch check would report as its own
+        if (device < 0 || device >= n) throw Error(SS_ERR_DEVICE, "no HIP device " + std::to_string(device));
+        SS_HIP(hipSetDevice(device));
+        moved = true;
+    }
+    ~OnDevice() { if (moved) (void)hipSetDevice(before); }
+};
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// null = fine, else what is wrong
+const char* bad_cache(const ss_kv_cache& c) {
+    if (c.kind != SS_KV_SAME && c.kind != SS_KV_E4M3 && c.kind != SS_KV_INT8) return "unknown kind";
+    if (c.dtype != SS_DTYPE_F16 && c.dtype != SS_DTYPE_BF16) return "dtype must be SS_DTYPE_F16 or SS_DTYPE_BF16";
+    if (c.head_dim != 64 && c.head_dim != 128) return "head_dim must be 64 or 128";
+    if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1))) return "page_size must be a power of two from 16 to 256";
+    if (c.n_pages <= 0 || c.n_kv_heads <= 0 || c.n_kv_heads > 4096) return "n_pages and n_kv_heads must be positive (at most 4096 heads)";
+    const int64_t rows = (int64_t)c.n_kv_heads * c.page_size;
+    if (c.page_stride < rows * c.head_dim || c.page_stride % 16 || c.page_stride > (int64_t)1 << 40) return "page_stride must hold a page and be a multiple of 16";
+    if (!c.k || !c.v || !aligned(c.k, 16) || !aligned(c.v, 16)) return "k and v must be 16-byte aligned device pointers";
+    if (c.kind != SS_KV_SAME) {
+        if (!c.k_scale || !c.v_scale || !aligned(c.k_scale, 16) || !aligned(c.v_scale, 16)) return "an 8-bit cache needs 16-byte aligned k_scale and v_scale";
+        if (c.scale_stride < rows || c.scale_stride % 16 || c.scale_stride > (int64_t)1 << 40) return "scale_stride must hold a page's rows and be a multiple of 16";
+    }
+    return nullptr;
+}
+const char* bad_batch(const ss_kv_batch& b, const ss_kv_cache& c) {
+    if (b.n_seqs < 0 || b.n_tokens < 0 || b.max_new < 0 || b.min_new < 0 || b.max_len < 0) return "negative size";
+    if (b.n_seqs > 1 << 20 || b.n_tokens > 1 << 28) return "too many sequences or tokens";
+    if (b.max_pages <= 0 || (int64_t)b.max_pages * c.page_size >= (int64_t)1 << 30) return "max_pages * page_size must lie in (0, 2^30)";
+    if (b.table_stride < b.max_pages) return "table_stride is smaller than max_pages";
+    if (b.n_seqs > 0 && (!b.page_table || !b.q_start || !b.kv_len)) return "null page_table, q_start or kv_len";
+    if (!aligned(b.page_table, 4) || !aligned(b.q_start, 4) || !aligned(b.kv_len, 4)) return "page_table, q_start and kv_len must be 4-byte aligned";
+    if (b.min_new > b.max_new) return "min_new is larger than max_new";
+    return nullptr;
+}
+const char* bad_rows(const ss_kv_rows* r, int n_tokens, int heads, int dim, bool written) {
+    if (!r) return "null rows";
+    if (n_tokens == 0) return nullptr;
+    if (!r->p || !aligned(r->p, 16)) return "token rows must be 16-byte aligned device pointers";
+    if (r->row_stride % 8 || r->head_stride % 8 || r->row_stride < 0 || r->head_stride < 0) return "row_stride and head_stride must be non-negative multiples of 8";
+    if (r->row_stride > (int64_t)1 << 32 || r->head_stride > (int64_t)1 << 32) return "stride too large";
+    if (written) {
+        const bool head_inside = (heads == 1 || r->head_stride >= dim) && (n_tokens == 1 || r->row_stride >= (int64_t)(heads - 1) * r->head_stride + dim);
+        const bool row_inside = (n_tokens == 1 || r->row_stride >= dim) && (heads == 1 || r->head_stride >= (int64_t)(n_tokens - 1) * r->row_stride + dim);
+        if (!head_inside && !row_inside) return "rows that are written must not overlap";
+    }
+    return nullptr;
+}
+const char* bad_heads(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads) {
+    if (n_heads <= 0 || n_heads % c.n_kv_heads || n_heads > 1 << 16) return "n_heads must be a multiple of n_kv_heads (at most 65536)";
+    if ((int64_t)b.max_new * (n_heads / c.n_kv_heads) >= (int64_t)1 << 30 || (int64_t)b.n_tokens * n_heads >= (int64_t)1 << 32) return "too many query rows";
+    // workgroups of either kernel (at most 64 key ranges each)
+    if ((int64_t)b.n_seqs * c.n_kv_heads * (((int64_t)b.max_new * (n_heads / c.n_kv_heads) + 63) / 64) >= (int64_t)1 << 24) return "too many sequences x heads x query tiles";
+    return nullptr;
+}
+int refuse(const char* who, const char* why) { return fail(SS_ERR_ARG, std::string(who) + ": " + why); }
+}  // namespace
+
+extern "C" {
+
+int32_t ss_sizeof_kv_cache(void) { return (int32_t)sizeof(ss_kv_cache); }
+int32_t ss_sizeof_kv_batch(void) { return (int32_t)sizeof(ss_kv_batch); }
+int32_t ss_sizeof_kv_rows(void) { return (int32_t)sizeof(ss_kv_rows); }
+int32_t ss_sizeof_sample_rows_args(void) { return (int32_t)sizeof(ss_sample_rows_args); }
+
+int ss_kv_append(const ss_kv_cache* c, const ss_kv_batch* b, const ss_kv_rows* k, const ss_kv_rows* v, int32_t device, void* stream) {
+    SS_TRY
+    if (!c || !b) return refuse("ss_kv_append", "null argument");
+    const char* why = bad_cache(*c);
+    if (!why) why = bad_batch(*b, *c);
+    if (!why) why = bad_rows(k, b->n_tokens, c->n_kv_heads, c->head_dim, false);
+    if (!why) why = bad_rows(v, b->n_tokens, c->n_kv_heads, c->head_dim, false);
+    if (why) return refuse("ss_kv_append", why);
+    OnDevice on(device);
+    launch_kv_append(*c, *b, *k, *v, (hipStream_t)stream);
+    return SS_OK;
+    SS_CATCH
+}
+int ss_kv_read(const ss_kv_cache* c, const ss_kv_batch* b, const ss_kv_rows* k, const ss_kv_rows* v, int32_t device, void* stream) {
+    SS_TRY
+    if (!c || !b) return refuse("ss_kv_read", "null argument");
+    const char* why = bad_cache(*c);
+    if (!why) why = bad_batch(*b, *c);
+    if (!why) why = bad_rows(k, b->n_tokens, c->n_kv_heads, c->head_dim, true);
+    if (!why) why = bad_rows(v, b->n_tokens, c->n_kv_heads, c->head_dim, true);
+    if (why) return refuse("ss_kv_read", why);
+    OnDevice on(device);
+    launch_kv_read(*c, *b, *k, *v, (hipStream_t)stream);
+    return SS_OK;
+    SS_CATCH
+}
+int64_t ss_kv_attention_workspace(const ss_kv_cache* c, const ss_kv_batch* b, int32_t n_heads) {
+    SS_TRY
+    if (!c || !b) return refuse("ss_kv_attention_workspace", "null argument");
+    const char* why = bad_cache(*c);
+    if (!why) why = bad_batch(*b, *c);
+    if (!why) why = bad_heads(*c, *b, n_heads);
+    if (why) return refuse("ss_kv_attention_workspace", why);
+    return kv_attention_plan(*c, *b, n_heads).workspace;
+    SS_CATCH
+}
+int ss_kv_attention(const ss_kv_cache* c, const ss_kv_batch* b, const ss_kv_rows* q, int32_t n_heads, float scale, int32_t causal, const ss_kv_rows* out, float* lse,
+                    void* workspace, int64_t workspace_bytes, int32_t device, void* stream) {
+    SS_TRY
+    if (!c || !b) return refuse("ss_kv_attention", "null argument");
+    const char* why = bad_cache(*c);
+    if (!why) why = bad_batch(*b, *c);
+    if (!why) why = bad_heads(*c, *b, n_heads);
+    if (!why) why = bad_rows(q, b->n_tokens, n_heads, c->head_dim, false);
+    if (!why) why = bad_rows(out, b->n_tokens, n_heads, c->head_dim, true);
+    if (!why && !(scale == scale && scale - scale == 0.0f)) why = "scale must be finite";
+    if (!why && !aligned(lse, 4)) why = "lse must be 4-byte aligned";
+    if (why) return refuse("ss_kv_attention", why);
+    const int64_t need = kv_attention_plan(*c, *b, n_heads).workspace;
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
+        return fail(workspace && aligned(workspace, 16) ? SS_ERR_BUFFER : SS_ERR_ARG,
+                    "ss_kv_attention: needs " + std::to_string(need) + " bytes of 16-byte aligned workspace, got " + std::to_string(workspace ? workspace_bytes : 0));
+    OnDevice on(device);
+    launch_kv_attention(*c, *b, *q, n_heads, scale, causal != 0, *out, lse, workspace, (hipStream_t)stream);
+    return SS_OK;
+    SS_CATCH
+}
+int ss_sample_rows(const ss_sample_rows_args* a, int32_t device, void* stream) {
+    SS_TRY
+    if (!a) return refuse("ss_sample_rows", "null argument");
+    const int size = a->dtype == SS_DTYPE_F32 ? 4 : 2;
+    const char* why = nullptr;
+    if (a->dtype != SS_DTYPE_F32 && a->dtype != SS_DTYPE_F16 && a->dtype != SS_DTYPE_BF16) why = "dtype must be SS_DTYPE_F32, SS_DTYPE_F16 or SS_DTYPE_BF16";
+    else if (a->n_rows < 0 || a->n_rows > 1 << 24) why = "n_rows must lie in [0, 2^24]";
+    else if (a->n_vocab <= 0 || a->n_vocab > 1 << 20) why = "n_vocab must lie in [1, 2^20]";
+    else if (a->row_stride < a->n_vocab || a->row_stride > (int64_t)1 << 40) why = "row_stride is smaller than n_vocab";
+    else if (a->n_rows > 0 && (!a->logits || !a->u || !a->id)) why = "null logits, u or id";
+    else if (!aligned(a->logits, size) || !aligned(a->u, 8) || !aligned(a->temperature, 4) || !aligned(a->top_k, 4) || !aligned(a->top_p, 4) || !aligned(a->min_p, 4) ||
+             !aligned(a->id, 4) || !aligned(a->p, 4) || !aligned(a->logprob, 4) || !aligned(a->n_kept, 4)) why = "misaligned pointer";
+    if (why) return refuse("ss_sample_rows", why);
+    OnDevice on(device);
+    launch_sample_rows(*a, (hipStream_t)stream);
+    return SS_OK;
+    SS_CATCH
 }
 
 }  // extern "C"

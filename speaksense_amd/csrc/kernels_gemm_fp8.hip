@@ -124,7 +124,7 @@ __device__ __forceinline__ void f8_epilogue(const GemmF8Desc& g, f32x16 (&acc)[2
 #pragma unroll
                 for (int gq = 0; gq < 4; gq++)
 #pragma unroll
-                    for (int r = 0; r < 4; r += 2) {   // packed-f32 GELU (gemm_common.h gelu_tanh_pk): two elements per VALU instruction
+                    for (int r = 0; r < 4; r += 2) {   // two elements at a time (gemm_common.h gelu_tanh_pk)
                         f32x2 t = {acc[ni][mi][gq * 4 + r], acc[ni][mi][gq * 4 + r + 1]};
                         if (std::is_same<T, f16>::value && g.gelu_f16_in) t = gelu_tanh_pk<true>(t); else t = gelu_tanh_pk<false>(t);
                         v[ni][gq][r] = t[0]; v[ni][gq][r + 1] = t[1];

@@ -1,0 +1,927 @@
+// Paged key / value cache for gfx950: append with quantisation, read back, attention of a chunk of new tokens.
+//
+// Cache of one layer: k and v are [n_pages][n_kv_heads][page_size][head_dim] codes, one scale per (page, head, row) beside 8-bit codes:
+//   same   f16 / bf16 as the tokens
+//   e4m3   code = RNE_e4m3(x 2^(127 - e)), e = E8M0 byte with amax / 2^(e - 127) <= 448 (the format of the fp8 engine's cross cache)
+//   int8   s = amax / 127 (IEEE), code = rint(x / s)
+// A sequence s of the step has n_s = q_start[s + 1] - q_start[s] new tokens, the last n_s of its kv_len[s] positions; position p lies in row
+// p % page_size of page page_table[s][p / page_size].  Every index that comes from device memory is checked here before it is used: a page number
+// outside [0, n_pages) holds nothing (its keys are masked, reads give zeros, writes are dropped), spans of q_start outside the token rows are empty.
+#include <algorithm>
+#include <type_traits>
+
+#include "gemm_common.h"
+#include "ops.h"
+#include "wave_ops.h"
+
+namespace ss {
+namespace {
+
+enum { K_F16 = 0, K_BF16 = 1, K_E4M3 = 2, K_I8 = 3 };   // what the cache holds
+
+struct KvArgs {
+    char *k, *v, *ks, *vs;
+    long page_bytes, sc_stride;          // between pages: bytes of codes, elements of scales
+    const int *table, *q_start, *kv_len;
+    long table_stride;
+    int n_pages, page_shift, H, max_pages, n_seqs, n_tokens;
+};
+
+struct Span { int q0, n_new, len, pos0; };   // first token row, new tokens, positions held, position of the first new token
+__device__ __forceinline__ Span seq_span(const KvArgs& a, int s) {
+    Span r;
+    r.q0 = a.q_start[s];
+    const int q1 = a.q_start[s + 1];
+    r.n_new = r.q0 >= 0 && q1 > r.q0 && q1 <= a.n_tokens ? q1 - r.q0 : 0;
+    const int held = max(a.kv_len[s], 0);
+    r.len = min(held, a.max_pages << a.page_shift);      // the host has checked that the product fits 31 bits
+    r.pos0 = held - r.n_new;
+    return r;
+}
+__device__ __forceinline__ int page_at(const KvArgs& a, int s, int page) {   // page index inside the sequence -> page of the cache, or -1
+    if (page < 0 || page >= a.max_pages) return -1;
+    const int p = a.table[(long)s * a.table_stride + page];
+    return p < 0 || p >= a.n_pages ? -1 : p;
+}
+// The sequence of token row t: 64 boundaries a step.  Any contents of q_start give an index in [-1, n_seqs]; the caller checks the span itself.
+__device__ __forceinline__ int find_seq(const int* qs, int n_seqs, int t) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = n_seqs + 1;
+    while (len > 64) {
+        const int step = (len + 63) >> 6, i = (lane + 1) * step - 1;
+        const bool below = i < len && qs[lo + i] <= t;
+        const int c = __popcll(__ballot(below));
+        lo += c * step;
+        len = min(step, len - c * step);
+    }
+    const bool below = lane < len && qs[lo + lane] <= t;
+    return lo + __popcll(__ballot(below)) - 1;
+}
+
+// ---------------------------------------------------------------------------------------------
+// append / read: one workgroup per token row and 256 / (head_dim / 8) of its 2 H key and value rows; 8 elements (16 bytes) a lane.
+// Bound by HBM: 2 bytes of tokens and 1 or 2 of codes per element, once each.
+// ---------------------------------------------------------------------------------------------
+template <int LPR> __device__ __forceinline__ unsigned lanes_umax(unsigned v) {   // over the LPR lanes of a row
+#define SS_DPP_UMAX(CTRL) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false))
+    SS_DPP_UMAX(kDppXor1); SS_DPP_UMAX(kDppXor2); SS_DPP_UMAX(kDppHalfMirror);
+    if (LPR == 16) SS_DPP_UMAX(kDppRor8);
+#undef SS_DPP_UMAX
+    return v;
+}
+
+template <typename T, int KIND, int D>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, const T* __restrict__ kn, long k_row, long k_head, const T* __restrict__ vn, long v_row, long v_head) {
+    typedef typename Mfma<T>::V8 V8;
+    constexpr int LPR = D / 8;
+    const int t = blockIdx.x;
+    const int s = find_seq(a.q_start, a.n_seqs, t);
+    if (s < 0 || s >= a.n_seqs) return;                  // rows behind the last sequence
+    const Span sp = seq_span(a, s);
+    if (t < sp.q0 || t >= sp.q0 + sp.n_new) return;
+    const int pos = sp.pos0 + (t - sp.q0);
+    if (pos < 0) return;
+    const int page = page_at(a, s, pos >> a.page_shift);
+    if (page < 0) return;
+    const int item = blockIdx.y * 256 + threadIdx.x, r = item / LPR, c = item % LPR;
+    if (r >= 2 * a.H) return;
+    const bool is_v = r >= a.H;
+    const int h = is_v ? r - a.H : r;
+    const T* src = is_v ? vn + (long)t * v_row + (long)h * v_head : kn + (long)t * k_row + (long)h * k_head;
+    const V8 x = *(const V8*)(src + c * 8);
+    const long slot = ((long)h << a.page_shift) + (pos & ((1 << a.page_shift) - 1));   // row inside the page
+    char* dst = (is_v ? a.v : a.k) + (long)page * a.page_bytes;
+    if constexpr (KIND == K_F16 || KIND == K_BF16) {
+        *(V8*)(dst + (slot * D + c * 8) * 2) = x;
+    } else {
+        float f[8];
+        unsigned top = 0;      // the largest magnitude as bits: a NaN outranks every number, so a row that holds one reads back as NaN
+#pragma unroll
+        for (int i = 0; i < 8; i++) { f[i] = (float)x[i]; top = max(top, __float_as_uint(f[i]) & 0x7fffffffu); }
+        top = lanes_umax<LPR>(top);
+        uint2 code;
+        char* sc = is_v ? a.vs : a.ks;
+        const long at = (long)page * a.sc_stride + slot;
+        if constexpr (KIND == K_E4M3) {
+            const int e = e8m0_for_amax(__uint_as_float(top));
+            const float m = pow2_neg_of_e8m0(e);
+            code.x = pack_e4m3x4(f[0] * m, f[1] * m, f[2] * m, f[3] * m);
+            code.y = pack_e4m3x4(f[4] * m, f[5] * m, f[6] * m, f[7] * m);
+            if (c == 0) sc[at] = (char)e;
+        } else {
+            const float s8 = __uint_as_float(top) / 127.0f, by = s8 > 0.0f ? s8 : 1.0f;
+            unsigned b[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) b[i] = (unsigned)(int)fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f) & 0xffu;
+            code.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+            code.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
+            if (c == 0) ((float*)sc)[at] = s8;
+        }
+        *(uint2*)(dst + slot * D + c * 8) = code;
+    }
+}
+
+__device__ __forceinline__ float i8_at(unsigned w, int i) { return (float)(int)(signed char)(w >> (8 * i)); }
+
+template <typename T, int KIND, int D>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, T* __restrict__ ko, long k_row, long k_head, T* __restrict__ vo, long v_row, long v_head) {
+    typedef typename Mfma<T>::V8 V8;
+    constexpr int LPR = D / 8;
+    const int t = blockIdx.x;
+    const int s = find_seq(a.q_start, a.n_seqs, t);
+    if (s < 0 || s >= a.n_seqs) return;
+    const Span sp = seq_span(a, s);
+    if (t < sp.q0 || t >= sp.q0 + sp.n_new) return;
+    const int pos = sp.pos0 + (t - sp.q0);
+    const int page = pos < 0 ? -1 : page_at(a, s, pos >> a.page_shift);
+    const int item = blockIdx.y * 256 + threadIdx.x, r = item / LPR, c = item % LPR;
+    if (r >= 2 * a.H) return;
+    const bool is_v = r >= a.H;
+    const int h = is_v ? r - a.H : r;
+    V8 x;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (T)0.0f;
+    if (page >= 0) {
+        const long slot = ((long)h << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+        const char* src = (is_v ? a.v : a.k) + (long)page * a.page_bytes;
+        if constexpr (KIND == K_F16 || KIND == K_BF16) {
+            x = *(const V8*)(src + (slot * D + c * 8) * 2);
+        } else {
+            const uint2 code = *(const uint2*)(src + slot * D + c * 8);
+            const char* sc = is_v ? a.vs : a.ks;
+            const long at = (long)page * a.sc_stride + slot;
+            float f[8], m;
+            if constexpr (KIND == K_E4M3) {
+                m = __uint_as_float((unsigned)(unsigned char)sc[at] << 23);
+#define SS_F8(I, W, B) f[I] = __builtin_amdgcn_cvt_f32_fp8(W, B)
+                SS_F8(0, code.x, 0); SS_F8(1, code.x, 1); SS_F8(2, code.x, 2); SS_F8(3, code.x, 3);
+                SS_F8(4, code.y, 0); SS_F8(5, code.y, 1); SS_F8(6, code.y, 2); SS_F8(7, code.y, 3);
+#undef SS_F8
+            } else {
+                m = ((const float*)sc)[at];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { f[i] = i8_at(code.x, i); f[4 + i] = i8_at(code.y, i); }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = (T)(f[i] * m);
+        }
+    }
+    T* dst = is_v ? vo + (long)t * v_row + (long)h * v_head : ko + (long)t * k_row + (long)h * k_head;
+    *(V8*)(dst + c * 8) = x;
+}
+
+// ---------------------------------------------------------------------------------------------
+// attention: o_q = sum_j p_qj v_j / sum_j p_qj, p_qj = exp2(x_qj - m_q), x_qj = scale log2(e) q.k_j, over j < limit_q.
+//
+// Both kernels compute S^T = K Q^T with mfma 16x16x32 (A = 16 keys, B = 16 query rows), so a lane owns one query row (lane & 15) and, of every 16
+// keys, rows 4 g .. 4 g + 3 (g = lane >> 4).  Two such blocks give it 8 keys = its B operand of the next product O^T = V^T P^T: the contraction index
+// (g, j) stands for key 16 (j >> 2) + 4 g + (j & 3) on both sides, so the probabilities never leave the registers.  The A operand of that product
+// wants, per lane, 8 keys of one column; a lane reads D/16 neighbouring columns of its 8 keys (whole lines across the 16 lanes) and turns that
+// little block with v_perm: MFMA number jj takes column (D/16) (lane & 15) + jj.  No transposed copy of V exists anywhere.
+//
+// 8-bit caches: codes enter the MFMA as f16 (exact: |code| <= 448) whatever the tokens' type; a key's scale multiplies its score in f32, a value's
+// scale multiplies its probability, relative to a running power of two (sref) near the largest scale seen, so that no term leaves f16's range.
+// bf16 queries are brought to f16 by a power of two of their own (exact but for elements below 2^-24 of the row's largest).
+//
+// m_q need not be the maximum, only near it: it moves when a score exceeds it by more than 2^8 (p then is at most 2^8, in f16 as in bf16), which
+// leaves most tiles without a reduction across lanes and without rescaling O.
+// ---------------------------------------------------------------------------------------------
+struct AttnArgs {
+    const void* q; long q_row, q_head;
+    void* out; long o_row, o_head;
+    float* lse;                        // [n_tokens][heads] or null
+    float* part; float2* part_ml;      // [n_tokens][heads][splits][D], [n_tokens][heads][splits]
+    float c2;                          // scale * log2(e)
+    int G, causal, splits, split_keys; // query heads per key head; key ranges and their length (a multiple of 128)
+    int all, nq;                       // tile kernel: also the sequences of at most 16 query rows; query tiles per (sequence, head)
+};
+
+constexpr float kInf = __builtin_huge_valf();
+constexpr float kSlack = 8.0f;         // log2 of the largest probability relative to m
+
+template <int KIND> struct Held;       // what the MFMA multiplies, and bytes of an element
+template <> struct Held<K_F16> { typedef f16 M; static constexpr int B = 2; };
+template <> struct Held<K_BF16> { typedef bf16 M; static constexpr int B = 2; };
+template <> struct Held<K_E4M3> { typedef f16 M; static constexpr int B = 1; };
+template <> struct Held<K_I8> { typedef f16 M; static constexpr int B = 1; };
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ unsigned perm(unsigned hi, unsigned lo, unsigned sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+
+// four codes -> two f16 pairs.  int8: byte u = code + 128 under the byte 0x64 is the f16 number 1024 + u; minus 1152 gives the code, exactly
+__device__ __forceinline__ unsigned f16_less_1152(unsigned w) {
+    const h16x2 k = {(f16)1152.0f, (f16)1152.0f};
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(h16x2, w) - k);
+}
+template <int KIND> __device__ __forceinline__ void codes_to_f16(unsigned w, unsigned* o) {
+    if constexpr (KIND == K_E4M3) {
+        o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+        o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+    } else {
+        w ^= 0x80808080u;
+        o[0] = f16_less_1152(perm(0x64646464u, w, 0x04010400u));
+        o[1] = f16_less_1152(perm(0x64646464u, w, 0x04030402u));
+    }
+}
+
+// the 16 query rows of one column tile as B operands; returns the power of two that was taken out of this lane's row.  `dim0(s)`: first of the 8
+// dims that this lane's group contributes to k-step s
+template <typename T, typename M, int D, bool PAIRED>
+__device__ __forceinline__ float load_q(const T* q, bool ok, int g, typename Mfma<M>::V8* qf) {
+    typedef typename Mfma<T>::V8 TV8;
+    TV8 x[D / 32];
+#pragma unroll
+    for (int s = 0; s < D / 32; s++) {
+        const int dim = PAIRED ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+        if (ok) x[s] = *(const TV8*)(q + dim);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[s][i] = (T)0.0f;
+    }
+    float back = 1.0f;
+    if constexpr (std::is_same<T, M>::value) {
+#pragma unroll
+        for (int s = 0; s < D / 32; s++) qf[s] = x[s];
+    } else {
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < D / 32; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf((float)x[s][i]));
+        top = rows_max(top);
+        const unsigned e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+        const float m = __uint_as_float((254u - e) << 23);
+        back = __uint_as_float(e << 23);
+#pragma unroll
+        for (int s = 0; s < D / 32; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) qf[s][i] = (M)((float)x[s][i] * m);
+    }
+    return back;
+}
+
+// A operand of O^T += V^T P^T from the D/16 columns x 8 keys block a lane holds (DW dwords per key)
+template <typename M, int KIND, int D> struct VBlock {
+    static constexpr int DW = D / 16 * Held<KIND>::B / 4;
+    unsigned w[8][DW];
+    __device__ __forceinline__ void frags(typename Mfma<M>::V8* f) const {
+        u32x4* o = (u32x4*)f;
+        if constexpr (Held<KIND>::B == 2) {
+#pragma unroll
+            for (int d = 0; d < DW; d++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    o[2 * d][t] = perm(w[2 * t + 1][d], w[2 * t][d], 0x05040100u);
+                    o[2 * d + 1][t] = perm(w[2 * t + 1][d], w[2 * t][d], 0x07060302u);
+                }
+        } else if constexpr (KIND == K_E4M3) {
+#pragma unroll
+            for (int d = 0; d < DW; d++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    unsigned x[2], y[2];
+                    codes_to_f16<KIND>(w[2 * t][d], x);
+                    codes_to_f16<KIND>(w[2 * t + 1][d], y);
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {
+                        o[4 * d + 2 * p][t] = perm(y[p], x[p], 0x05040100u);
+                        o[4 * d + 2 * p + 1][t] = perm(y[p], x[p], 0x07060302u);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DW; d++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const unsigned x = w[2 * t][d] ^ 0x80808080u, y = w[2 * t + 1][d] ^ 0x80808080u;
+                    const unsigned lo = perm(y, x, 0x05010400u), hi = perm(y, x, 0x07030602u);   // (x0 y0 x1 y1), (x2 y2 x3 y3)
+                    o[4 * d][t] = f16_less_1152(perm(0x64646464u, lo, 0x04010400u));
+                    o[4 * d + 1][t] = f16_less_1152(perm(0x64646464u, lo, 0x04030402u));
+                    o[4 * d + 2][t] = f16_less_1152(perm(0x64646464u, hi, 0x04010400u));
+                    o[4 * d + 3][t] = f16_less_1152(perm(0x64646464u, hi, 0x04030402u));
+                }
+        }
+    }
+};
+
+// Online softmax state of one column tile (a lane's query row), and the step for 32 keys
+template <typename M, bool SCALED, int D> struct Row {
+    float m = -kInf, l = 0.0f;         // l: this lane's keys only, summed over the four groups at the end
+    f32x4 o[D / 16];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[i] = (f32x4){0, 0, 0, 0};
+    }
+    // x[8]: scores in log2 units (-inf where masked); returns the probabilities' B operand; v[8]: value scales / sref
+    __device__ __forceinline__ typename Mfma<M>::V8 probs(const float* x, const float* v) {
+        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__ballot(top > m + kSlack)) {
+            const float mn = fmaxf(m, rows_max(top)), ref = mn == -kInf ? 0.0f : mn;
+            const float a = __builtin_amdgcn_exp2f(m - ref);
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) o[i] *= a;
+        }
+        const float ref = m == -kInf ? 0.0f : m;
+        typename Mfma<M>::V8 p;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float e = __builtin_amdgcn_exp2f(x[j] - ref);
+            l += e;
+            p[j] = (M)(SCALED ? e * v[j] : e);
+        }
+        return p;
+    }
+    __device__ __forceinline__ void add(const typename Mfma<M>::V8* vf, typename Mfma<M>::V8 p) {
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[i] = Mfma<M>::mma(vf[i], p, o[i]);
+    }
+};
+
+// the running power of two near the largest value scale; one per wave
+struct ScaleRef {
+    float ref = 0.0f;
+    // returns what O has to be multiplied by (1 when nothing moved)
+    __device__ __forceinline__ bool moves(const float* v, float* by) {
+        const float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+        if (!__ballot(top > ref * 64.0f)) return false;
+        const float n = __uint_as_float(__float_as_uint(fmaxf(wave_max(top), ref)) & 0x7f800000u);
+        *by = n > 0.0f ? ref / n : 0.0f;
+        ref = n;
+        return true;
+    }
+    __device__ __forceinline__ float inv() const { return ref > 0.0f ? 1.0f / ref : 0.0f; }
+};
+
+// a finished row's output: acc[D/16] columns from `col` on of head row `out`
+template <typename T, int N> __device__ __forceinline__ void store_cols(T* p, const float* x) {
+    if constexpr (N == 4) {
+        typename Mfma<T>::V4 y;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = (T)x[i];
+        *(typename Mfma<T>::V4*)p = y;
+    } else {
+        typename Mfma<T>::V8 y;
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = (T)x[i];
+        *(typename Mfma<T>::V8*)p = y;
+    }
+}
+
+// ---- few query rows (n_new G <= 16): grid (sequences x splits, key heads); the 4 waves of a workgroup take every fourth 32-key tile of its key
+// range straight from memory into registers (the next tile's loads fly while one is computed) and merge at the end.  HBM-bound: with G <= 16 the
+// MFMA issues of a tile take ~1/10 of the time its bytes need at the card's rate, so the 15 idle columns of a one-head row cost nothing. ----
+template <int KIND, int D> struct KvTile {
+    static constexpr int B = Held<KIND>::B, KN = D * B / 64;   // 16-byte pieces of a key row per lane
+    u32x4 k[2][KN];
+    VBlock<typename Held<KIND>::M, KIND, D> v;
+    float ks[8], vs[8];
+    int page[2];
+
+    __device__ __forceinline__ void load(const KvArgs& a, int h, int key0, int p0, int p1, int lane) {
+        const int m = lane & 15, g = lane >> 4;
+        page[0] = p0; page[1] = p1;
+        const int mask = (1 << a.page_shift) - 1;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int p = max(page[b], 0), r0 = (key0 + 16 * b) & mask;     // 16 keys share a page
+            const long row = ((long)h << a.page_shift) + r0;
+            const char* kp = a.k + (long)p * a.page_bytes + row * (D * B);
+            const char* vp = a.v + (long)p * a.page_bytes + row * (D * B);
+#pragma unroll
+            for (int i = 0; i < KN; i++) k[b][i] = *(const u32x4*)(kp + m * (D * B) + 64 * i + 16 * g);
+            constexpr int DW = VBlock<typename Held<KIND>::M, KIND, D>::DW;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const char* src = vp + (4 * g + r) * (D * B) + m * (4 * DW);
+                if constexpr (DW == 1) v.w[4 * b + r][0] = *(const unsigned*)src;
+                else if constexpr (DW == 2) { const u32x2 t = *(const u32x2*)src; v.w[4 * b + r][0] = t[0]; v.w[4 * b + r][1] = t[1]; }
+                else {
+                    const u32x4 t = *(const u32x4*)src;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v.w[4 * b + r][i] = t[i];
+                }
+            }
+            const long at = (long)p * a.sc_stride + row + 4 * g;
+            if constexpr (KIND == K_E4M3) {
+                const unsigned x = *(const unsigned*)(a.ks + at), y = *(const unsigned*)(a.vs + at);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    ks[4 * b + r] = __uint_as_float((x >> (8 * r) & 255u) << 23);
+                    vs[4 * b + r] = __uint_as_float((y >> (8 * r) & 255u) << 23);
+                }
+            } else if constexpr (KIND == K_I8) {
+                const f32x4 x = *(const f32x4*)(a.ks + 4 * at), y = *(const f32x4*)(a.vs + 4 * at);
+#pragma unroll
+                for (int r = 0; r < 4; r++) { ks[4 * b + r] = x[r]; vs[4 * b + r] = y[r]; }
+            }
+        }
+    }
+};
+
+template <typename T, int KIND, int D>
+__global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) {
+    typedef typename Held<KIND>::M M;
+    typedef typename Mfma<M>::V8 V8;
+    constexpr bool SCALED = Held<KIND>::B == 1;
+    constexpr int N = D / 16;
+    __shared__ float s_o[4][16][D];
+    __shared__ float s_m[4][16], s_l[4][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int h = blockIdx.y, s = blockIdx.x / t.splits, split = blockIdx.x % t.splits;
+    const Span sp = seq_span(a, s);
+    const int rows = sp.n_new * t.G;
+    if (rows == 0 || rows > 16) return;
+
+    const bool mine = c < rows;
+    const int tok = c / t.G, row = sp.q0 + (mine ? tok : 0), head = h * t.G + (mine ? c % t.G : 0);
+    const int limit = !mine ? 0 : t.causal ? max(0, min(sp.pos0 + tok + 1, sp.len)) : sp.len;     // keys this lane's query row sees
+    const int full = t.causal ? max(0, min(sp.pos0 + 1, sp.len)) : sp.len;                        // keys every row sees
+    V8 qf[D / 32];
+    const float back = load_q<T, M, D, SCALED>((const T*)t.q + (long)row * t.q_row + (long)head * t.q_head, mine, g, qf);
+    const float c2 = t.c2 * back;
+
+    const int lo = split * t.split_keys, hi = split == t.splits - 1 ? sp.len : min(sp.len, lo + t.split_keys);
+    const int n = hi > lo ? (hi - lo + 31) / 32 : 0, mine_n = n > wave ? (n - wave + 3) / 4 : 0;   // tiles of the range / of this wave
+    Row<M, SCALED, D> st;
+    st.clear();
+    ScaleRef sr;
+
+    int ids[2] = {-1, -1};             // lane i: the pages of this wave's tile i of the current 64
+    auto fetch_ids = [&](int first) {
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int key = lo + ((first + lane) * 4 + wave) * 32 + 16 * b;
+            ids[b] = first + lane < mine_n && key < hi ? page_at(a, s, key >> a.page_shift) : -1;
+        }
+    };
+    auto load = [&](KvTile<KIND, D>& x, int i) {
+        if ((i & 63) == 0) fetch_ids(i);
+        x.load(a, h, lo + (i * 4 + wave) * 32, __builtin_amdgcn_readlane(ids[0], i & 63), __builtin_amdgcn_readlane(ids[1], i & 63), lane);
+    };
+    auto compute = [&](KvTile<KIND, D>& x, int i) {
+        const int key0 = lo + (i * 4 + wave) * 32;
+        float sc[8];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            f32x4 z = {0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) {
+                V8 kf;
+                if constexpr (!SCALED) kf = __builtin_bit_cast(V8, x.k[b][d]);
+                else {
+                    u32x4 w;
+                    unsigned o[2];
+                    codes_to_f16<KIND>(x.k[b][d >> 1][2 * (d & 1)], o); w[0] = o[0]; w[1] = o[1];
+                    codes_to_f16<KIND>(x.k[b][d >> 1][2 * (d & 1) + 1], o); w[2] = o[0]; w[3] = o[1];
+                    kf = __builtin_bit_cast(V8, w);
+                }
+                z = Mfma<M>::mma(kf, qf[d], z);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) sc[4 * b + r] = z[r] * (SCALED ? c2 * x.ks[4 * b + r] : c2);
+        }
+        if (key0 + 32 > full || x.page[0] < 0 || x.page[1] < 0) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+                const bool held = key < sp.len && x.page[j >> 2] >= 0;
+                if (!held || key >= limit) sc[j] = -kInf;
+                if (!held) {           // whatever lies there (it may be NaN): 0 x probability 0
+#pragma unroll
+                    for (int d = 0; d < x.v.DW; d++) x.v.w[j][d] = 0;
+                    x.vs[j] = 0.0f;
+                }
+            }
+        }
+        if constexpr (SCALED) {
+            float by;
+            if (sr.moves(x.vs, &by))
+#pragma unroll
+                for (int k = 0; k < N; k++) st.o[k] *= by;
+            const float inv = sr.inv();
+#pragma unroll
+            for (int j = 0; j < 8; j++) x.vs[j] *= inv;
+        }
+        const V8 p = st.probs(sc, x.vs);
+        V8 vf[N];
+        x.v.frags(vf);
+        st.add(vf, p);
+    };
+    KvTile<KIND, D> x, y;
+    if (mine_n > 0) load(x, 0);
+    for (int i = 0; i < mine_n; i += 2) {
+        if (i + 1 < mine_n) load(y, i + 1);
+        compute(x, i);
+        if (i + 1 < mine_n) {
+            if (i + 2 < mine_n) load(x, i + 2);
+            compute(y, i + 1);
+        }
+    }
+
+    // merge the four waves
+    const float l = rows_sum(st.l);
+    if (lane < 16) { s_m[wave][c] = st.m; s_l[wave][c] = l; }
+    __syncthreads();
+    float M4 = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c]));
+    const float f = __builtin_amdgcn_exp2f(st.m - M4) * (SCALED ? sr.ref : 1.0f);
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int k = 0; k < N; k++) s_o[wave][c][N * (4 * g + r) + k] = M4 == -kInf ? 0.0f : st.o[k][r] * f;
+    __syncthreads();
+    const int oc = threadIdx.x >> 4, col = (threadIdx.x & 15) * N;
+    if (oc >= rows) return;
+    M4 = fmaxf(fmaxf(s_m[0][oc], s_m[1][oc]), fmaxf(s_m[2][oc], s_m[3][oc]));
+    float L = 0.0f, acc[N];
+#pragma unroll
+    for (int w = 0; w < 4; w++) L += M4 == -kInf ? 0.0f : s_l[w][oc] * __builtin_amdgcn_exp2f(s_m[w][oc] - M4);
+#pragma unroll
+    for (int k = 0; k < N; k++) acc[k] = (s_o[0][oc][col + k] + s_o[1][oc][col + k]) + (s_o[2][oc][col + k] + s_o[3][oc][col + k]);
+    const int orow = sp.q0 + oc / t.G, ohead = h * t.G + oc % t.G;
+    const long at = (long)orow * (a.H * t.G) + ohead;
+    if (t.splits == 1) {
+        const float inv = L > 0.0f ? 1.0f / L : L;         // no key: zeros (L is 0 or NaN here)
+#pragma unroll
+        for (int k = 0; k < N; k++) acc[k] *= inv;
+        store_cols<T, N>((T*)t.out + (long)orow * t.o_row + (long)ohead * t.o_head + col, acc);
+        if (t.lse && col == 0) t.lse[at] = L > 0.0f ? (M4 + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
+    } else {
+        float* o = t.part + (at * t.splits + split) * D + col;
+#pragma unroll
+        for (int k = 0; k < N; k++) o[k] = acc[k];
+        if (col == 0) t.part_ml[at * t.splits + split] = make_float2(M4, L);
+    }
+}
+
+// ---- many query rows: a workgroup of 4 waves owns 64 QC query rows of one (sequence, key head), each wave 16 QC of them; 64-key tiles of K and V go
+// through LDS as 16 bits (8-bit codes are converted once, on the way in), the next tile's loads fly while one is computed, one barrier a tile. ----
+template <typename T, int KIND, int D, int QC>
+__global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t) {
+    typedef typename Held<KIND>::M M;
+    typedef typename Mfma<M>::V8 V8;
+    constexpr bool SCALED = Held<KIND>::B == 1;
+    constexpr int N = D / 16, B = Held<KIND>::B;
+    // row pitches: the 16 key rows a wave's lanes read 16 bytes of each fall on 64 different banks, and so do two value rows 4 apart
+    constexpr int KP = D * 2 + 16, VP = D == 64 ? D * 2 + 32 : D * 2 + 16;
+    constexpr int kBuf = 64 * (KP + VP) + 512;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    int bid = blockIdx.x;
+    {   // consecutive workgroups land on different XCDs: give each XCD a contiguous range, so that the query tiles of one (sequence, head) share an L2
+        const int nwg = gridDim.x, q8 = nwg / 8, r8 = nwg % 8, xcd = bid % 8, idx = bid / 8;
+        bid = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + idx;
+    }
+    const int qb = t.nq - 1 - bid % t.nq;                  // causal: the longest first
+    bid /= t.nq;
+    const int split = bid % t.splits;
+    bid /= t.splits;
+    const int h = bid % a.H, s = bid / a.H;
+    const Span sp = seq_span(a, s);
+    const int rows = sp.n_new * t.G, r0 = qb * (64 * QC);
+    if (rows <= r0 || (rows <= 16 && !t.all)) return;
+
+    const int w0 = r0 + wave * (16 * QC);                  // this wave's first query row
+    int limit[QC], orow[QC], ohead[QC];
+    V8 qf[QC][D / 32];
+    float c2[QC];
+#pragma unroll
+    for (int i = 0; i < QC; i++) {
+        const int q = w0 + 16 * i + c, tok = q / t.G;
+        const bool ok = q < rows;
+        orow[i] = sp.q0 + (ok ? tok : 0);
+        ohead[i] = h * t.G + (ok ? q - tok * t.G : 0);
+        limit[i] = !ok ? 0 : t.causal ? max(0, min(sp.pos0 + tok + 1, sp.len)) : sp.len;
+        c2[i] = t.c2 * load_q<T, M, D, false>((const T*)t.q + (long)orow[i] * t.q_row + (long)ohead[i] * t.q_head, ok, g, qf[i]);
+    }
+    const int last = min(rows, r0 + 64 * QC) - 1;
+    const int end = t.causal ? max(0, min(sp.pos0 + last / t.G + 1, sp.len)) : sp.len;            // keys any row of the workgroup sees
+    const int wend = w0 >= rows ? 0 : t.causal ? max(0, min(sp.pos0 + (min(rows, w0 + 16 * QC) - 1) / t.G + 1, sp.len)) : sp.len;   // of the wave
+    const int full = t.causal ? max(0, min(sp.pos0 + w0 / t.G + 1, sp.len)) : sp.len;             // keys every row of the wave sees
+    const int lo = split * t.split_keys, hi = split == t.splits - 1 ? end : min(end, lo + t.split_keys);
+    const int n = hi > lo ? (hi - lo + 63) / 64 : 0;
+
+    Row<M, SCALED, D> st[QC];
+#pragma unroll
+    for (int i = 0; i < QC; i++) st[i].clear();
+    ScaleRef sr;
+
+    // staging: a row of codes is D B / 16 pieces of 16 bytes; thread -> rows tid / PR + i (256 / PR)
+    constexpr int PR = D * B / 16, RP = 256 / PR, NP = 64 / RP;
+    u32x4 gk[NP], gv[NP];
+    float gks = 0.0f, gvs = 0.0f;      // threads 0..63: the scales of the tile's rows
+    const int mask = (1 << a.page_shift) - 1;
+    auto fetch = [&](int i) {
+        const int key0 = lo + i * 64;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const int key = key0 + tid / PR + p * RP;
+            const int page = key < sp.len ? page_at(a, s, key >> a.page_shift) : -1;
+            const long off = (long)max(page, 0) * a.page_bytes + (((long)h << a.page_shift) + (key & mask)) * (D * B) + (tid % PR) * 16;
+            gk[p] = *(const u32x4*)(a.k + off);
+            gv[p] = *(const u32x4*)(a.v + off);
+            if (page < 0) { gk[p] = (u32x4){0, 0, 0, 0}; gv[p] = (u32x4){0, 0, 0, 0}; }     // whatever lies there must not meet a probability of 0
+        }
+        if constexpr (SCALED)
+            if (tid < 64) {
+                const int key = key0 + tid, page = key < sp.len ? page_at(a, s, key >> a.page_shift) : -1;
+                const long at = (long)max(page, 0) * a.sc_stride + ((long)h << a.page_shift) + (key & mask);
+                if constexpr (KIND == K_E4M3) {
+                    gks = __uint_as_float((unsigned)(unsigned char)a.ks[at] << 23);
+                    gvs = __uint_as_float((unsigned)(unsigned char)a.vs[at] << 23);
+                } else { gks = ((const float*)a.ks)[at]; gvs = ((const float*)a.vs)[at]; }
+                if (page < 0) { gks = 0.0f; gvs = 0.0f; }
+            }
+    };
+    auto put = [&](char* buf) {
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+            const int r = tid / PR + p * RP;
+            char *kd = buf + r * KP, *vd = buf + 64 * KP + r * VP;
+            if constexpr (!SCALED) {
+                *(u32x4*)(kd + (tid % PR) * 16) = gk[p];
+                *(u32x4*)(vd + (tid % PR) * 16) = gv[p];
+            } else {
+                u32x4 x[2];
+                unsigned o[2];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { codes_to_f16<KIND>(gk[p][i], o); x[i >> 1][2 * (i & 1)] = o[0]; x[i >> 1][2 * (i & 1) + 1] = o[1]; }
+                *(u32x4*)(kd + (tid % PR) * 32) = x[0];
+                *(u32x4*)(kd + (tid % PR) * 32 + 16) = x[1];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { codes_to_f16<KIND>(gv[p][i], o); x[i >> 1][2 * (i & 1)] = o[0]; x[i >> 1][2 * (i & 1) + 1] = o[1]; }
+                *(u32x4*)(vd + (tid % PR) * 32) = x[0];
+                *(u32x4*)(vd + (tid % PR) * 32 + 16) = x[1];
+            }
+        }
+        if constexpr (SCALED)
+            if (tid < 64) { ((float*)(buf + 64 * (KP + VP)))[tid] = gks; ((float*)(buf + 64 * (KP + VP)))[64 + tid] = gvs; }
+    };
+    auto holes = [&](int key0) {       // bit b: the 16 keys from key0 + 16 b on lie on a page that is not there
+        int bad = 0;
+#pragma unroll
+        for (int b = 0; b < 4; b++) bad |= key0 + 16 * b < sp.len && page_at(a, s, (key0 + 16 * b) >> a.page_shift) < 0 ? 1 << b : 0;
+        return bad;
+    };
+    if (n > 0) {
+        fetch(0);
+        put(smem);
+        if (n > 1) fetch(1);
+    }
+    __syncthreads();
+    for (int i = 0; i < n; i++) {
+        const char* buf = smem + (i & 1) * kBuf;
+        const int key0 = lo + i * 64;
+        if (key0 < wend) {
+            const int bad = holes(key0);
+            const bool edge = key0 + 64 > full || bad;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                float vs[8], ks[8];
+                if constexpr (SCALED) {
+                    const float* sc = (const float*)(buf + 64 * (KP + VP));
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const f32x4 x = *(const f32x4*)(sc + half * 32 + 16 * b + 4 * g), y = *(const f32x4*)(sc + 64 + half * 32 + 16 * b + 4 * g);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) { ks[4 * b + r] = x[r]; vs[4 * b + r] = y[r]; }
+                    }
+                    float by;
+                    if (sr.moves(vs, &by))
+#pragma unroll
+                        for (int j = 0; j < QC; j++)
+#pragma unroll
+                            for (int k = 0; k < N; k++) st[j].o[k] *= by;
+                    const float inv = sr.inv();
+#pragma unroll
+                    for (int j = 0; j < 8; j++) vs[j] *= inv;
+                }
+                float x[QC][8];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const char* kp = buf + (half * 32 + 16 * b + c) * KP + g * 16;
+                    V8 kf[D / 32];
+#pragma unroll
+                    for (int d = 0; d < D / 32; d++) kf[d] = *(const V8*)(kp + d * 64);
+#pragma unroll
+                    for (int j = 0; j < QC; j++) {
+                        f32x4 z = {0, 0, 0, 0};
+#pragma unroll
+                        for (int d = 0; d < D / 32; d++) z = Mfma<M>::mma(kf[d], qf[j][d], z);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) x[j][4 * b + r] = z[r] * (SCALED ? c2[j] * ks[4 * b + r] : c2[j]);
+                    }
+                }
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int key = key0 + half * 32 + 16 * (e >> 2) + 4 * g + (e & 3);
+                        const bool hole = bad >> (2 * half + (e >> 2)) & 1;
+#pragma unroll
+                        for (int j = 0; j < QC; j++)
+                            if (hole || key >= limit[j]) x[j][e] = -kInf;
+                    }
+                }
+                V8 p[QC];
+#pragma unroll
+                for (int j = 0; j < QC; j++) p[j] = st[j].probs(x[j], vs);
+                VBlock<M, KIND == K_BF16 ? K_BF16 : K_F16, D> vb;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const char* vp = buf + 64 * KP + (half * 32 + 16 * (e >> 2) + 4 * g + (e & 3)) * VP + c * (2 * N);
+                    if constexpr (N == 4) { const u32x2 w = *(const u32x2*)vp; vb.w[e][0] = w[0]; vb.w[e][1] = w[1]; }
+                    else {
+                        const u32x4 w = *(const u32x4*)vp;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) vb.w[e][q] = w[q];
+                    }
+                }
+                V8 vf[N];
+                vb.frags(vf);
+#pragma unroll
+                for (int j = 0; j < QC; j++) st[j].add(vf, p[j]);
+            }
+        }
+        if (i + 1 < n) {
+            put(smem + ((i + 1) & 1) * kBuf);              // last read before the barrier that ended tile i - 1
+            if (i + 2 < n) fetch(i + 2);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < QC; j++) {
+        const float L = rows_sum(st[j].l), mm = st[j].m;
+        if (w0 + 16 * j + c >= rows) continue;
+        const long at = (long)orow[j] * (a.H * t.G) + ohead[j];
+        const float u = SCALED ? sr.ref : 1.0f;
+        if (t.splits == 1) {
+            const float inv = (L > 0.0f ? 1.0f / L : L) * u;
+            T* o = (T*)t.out + (long)orow[j] * t.o_row + (long)ohead[j] * t.o_head;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float y[N];
+#pragma unroll
+                for (int k = 0; k < N; k++) y[k] = L == 0.0f ? 0.0f : st[j].o[k][r] * inv;
+                store_cols<T, N>(o + N * (4 * g + r), y);
+            }
+            if (t.lse && g == 0) t.lse[at] = L > 0.0f ? (mm + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
+        } else {
+            float* o = t.part + (at * t.splits + split) * D;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int k = 0; k < N; k++) o[N * (4 * g + r) + k] = L == 0.0f ? 0.0f : st[j].o[k][r] * u;
+            if (g == 0) t.part_ml[at * t.splits + split] = make_float2(mm, L);
+        }
+    }
+}
+
+// one wave per query row: join its key ranges.  `few`: rows of the few-row kernel (n_new G <= 16), else those of the tile kernel (`all`: every row)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t, int few) {
+    const int heads = a.H * t.G, lane = threadIdx.x & 63;
+    const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= (long)a.n_tokens * heads) return;
+    const int row = (int)(at / heads), head = (int)(at % heads);
+    const int s = find_seq(a.q_start, a.n_seqs, row);
+    if (s < 0 || s >= a.n_seqs) return;
+    const Span sp = seq_span(a, s);
+    if (row < sp.q0 || row >= sp.q0 + sp.n_new) return;
+    if (!t.all && (sp.n_new * t.G <= 16) != (few != 0)) return;
+    const float2 ml = lane < t.splits ? t.part_ml[at * t.splits + lane] : make_float2(-kInf, 0.0f);
+    const float m = wave_max(ml.x), f = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
+    const float L = wave_sum(ml.y * f);
+    constexpr int E = D / 64;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = 0.0f;
+    for (int i = 0; i < t.splits; i++) {
+        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
+        if (w == 0.0f) continue;
+        const float* o = t.part + (at * t.splits + i) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] += w * o[e];
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L;
+    T* o = (T*)t.out + (long)row * t.o_row + (long)head * t.o_head + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = (T)(acc[e] * inv);
+    if (t.lse && lane == 0) t.lse[at] = L > 0.0f ? (m + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
+}
+
+KvArgs kv_args(const ss_kv_cache& c, const ss_kv_batch& b) {
+    KvArgs a{};
+    a.k = (char*)c.k; a.v = (char*)c.v; a.ks = (char*)c.k_scale; a.vs = (char*)c.v_scale;
+    a.page_bytes = c.page_stride * (c.kind == SS_KV_SAME ? 2 : 1);
+    a.sc_stride = c.scale_stride;
+    a.table = b.page_table; a.q_start = b.q_start; a.kv_len = b.kv_len; a.table_stride = b.table_stride;
+    a.n_pages = c.n_pages; a.page_shift = __builtin_ctz((unsigned)c.page_size); a.H = c.n_kv_heads;
+    a.max_pages = b.max_pages; a.n_seqs = b.n_seqs; a.n_tokens = b.n_tokens;
+    return a;
+}
+
+// calls f(type tag, kind tag, dim tag) for the cache's combination
+template <int V> using Int = std::integral_constant<int, V>;
+template <typename F> void by_type(const ss_kv_cache& c, F f) {
+    auto dim = [&](auto t, auto k) { c.head_dim == 64 ? f(t, k, Int<64>()) : f(t, k, Int<128>()); };
+    const bool bf = c.dtype == SS_DTYPE_BF16;
+    if (c.kind == SS_KV_SAME) { if (bf) dim(bf16(), Int<K_BF16>()); else dim(f16(), Int<K_F16>()); }
+    else if (c.kind == SS_KV_E4M3) { if (bf) dim(bf16(), Int<K_E4M3>()); else dim(f16(), Int<K_E4M3>()); }
+    else { if (bf) dim(bf16(), Int<K_I8>()); else dim(f16(), Int<K_I8>()); }
+}
+
+int up(long a, long b) { return (int)((a + b - 1) / b); }
+
+}  // namespace
+
+void launch_kv_append(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& k, const ss_kv_rows& v, hipStream_t st) {
+    if (b.n_tokens == 0 || b.n_seqs == 0) return;
+    const dim3 grid(b.n_tokens, up(2l * c.n_kv_heads * (c.head_dim / 8), 256));
+    by_type(c, [&](auto t, auto kind, auto dim) {
+        typedef decltype(t) T;
+        kv_append_kernel<T, kind.value, dim.value><<<grid, 256, 0, st>>>(kv_args(c, b), (const T*)k.p, k.row_stride, k.head_stride, (const T*)v.p, v.row_stride, v.head_stride);
+    });
+    SS_LAUNCH_CHECK();
+}
+
+void launch_kv_read(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& k, const ss_kv_rows& v, hipStream_t st) {
+    if (b.n_tokens == 0 || b.n_seqs == 0) return;
+    const dim3 grid(b.n_tokens, up(2l * c.n_kv_heads * (c.head_dim / 8), 256));
+    by_type(c, [&](auto t, auto kind, auto dim) {
+        typedef decltype(t) T;
+        kv_read_kernel<T, kind.value, dim.value><<<grid, 256, 0, st>>>(kv_args(c, b), (T*)k.p, k.row_stride, k.head_stride, (T*)v.p, v.row_stride, v.head_stride);
+    });
+    SS_LAUNCH_CHECK();
+}
+
+KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads) {
+    KvPlan p{};
+    p.few_splits = p.tile_splits = 1;
+    if (b.n_seqs == 0 || b.n_tokens == 0 || b.max_new == 0) return p;
+    const int G = n_heads / c.n_kv_heads;
+    const long cap = (long)b.max_pages * c.page_size, keys = std::max(1l, b.max_len > 0 ? std::min((long)b.max_len, cap) : cap);
+    const long rows = (long)b.max_new * G, pairs = (long)b.n_seqs * c.n_kv_heads;
+    p.tile = rows > 16;
+    p.few = !p.tile || (long)std::max(b.min_new, 1) * G <= 16;
+    p.qc = rows <= 64 ? 1 : 2;
+    p.few_keys = p.tile_keys = (int)std::min(keys, 1l << 30);
+    auto cut = [&](long groups, long want, int least, int* splits, int* len) {   // as many key ranges as fill the card, none shorter than `least`
+        const long n = std::max(1l, std::min({(want + groups - 1) / groups, (keys + least - 1) / least, 64l}));
+        *len = (int)((keys + n * 128 - 1) / (n * 128) * 128);
+        *splits = (int)((keys + *len - 1) / *len);
+    };
+    if (p.few) cut(pairs, 1024, 256, &p.few_splits, &p.few_keys);
+    if (p.tile) cut(pairs * up(rows, 64 * p.qc), 512, 512, &p.tile_splits, &p.tile_keys);
+    const int n = std::max(p.few_splits, p.tile_splits);
+    if (n > 1) p.workspace = (int64_t)b.n_tokens * n_heads * n * (c.head_dim + 2) * 4;
+    return p;
+}
+
+void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& q, int n_heads, float scale, bool causal, const ss_kv_rows& out,
+                         float* lse, void* workspace, hipStream_t st) {
+    if (b.n_tokens == 0 || b.n_seqs == 0 || b.max_new == 0) return;
+    const KvPlan p = kv_attention_plan(c, b, n_heads);
+    const KvArgs a = kv_args(c, b);
+    AttnArgs t{};
+    t.q = q.p; t.q_row = q.row_stride; t.q_head = q.head_stride;
+    t.out = out.p; t.o_row = out.row_stride; t.o_head = out.head_stride;
+    t.lse = lse; t.c2 = scale * 1.44269504088896340736f; t.G = n_heads / c.n_kv_heads; t.causal = causal;
+    t.all = p.tile && !p.few;
+    by_type(c, [&](auto tt, auto kind, auto dim) {
+        typedef decltype(tt) T;
+        constexpr int K = kind.value, D = dim.value;
+        auto join = [&](int few) {
+            if (t.splits == 1) return;
+            kv_attn_join_kernel<T, D><<<up((long)b.n_tokens * n_heads, 4), 256, 0, st>>>(a, t, few);
+            SS_LAUNCH_CHECK();
+        };
+        auto part = [&](int splits, int keys) {            // the two kernels follow each other on the stream: they may share the workspace
+            t.splits = splits; t.split_keys = keys;
+            t.part = (float*)workspace;
+            t.part_ml = (float2*)((float*)workspace + (size_t)b.n_tokens * n_heads * splits * D);
+        };
+        if (p.few) {
+            part(p.few_splits, p.few_keys);
+            kv_attn_few_kernel<T, K, D><<<dim3(b.n_seqs * p.few_splits, c.n_kv_heads), 256, 0, st>>>(a, t);
+            SS_LAUNCH_CHECK();
+            join(1);
+        }
+        if (p.tile) {
+            part(p.tile_splits, p.tile_keys);
+            auto go = [&](auto qc) {
+                constexpr int QC = qc.value, smem = 2 * (64 * (D * 2 + 16 + (D == 64 ? D * 2 + 32 : D * 2 + 16)) + 512);
+                static std::atomic<uint64_t> once{0};
+                once_per_device(once, [&] { SS_HIP(hipFuncSetAttribute((const void*)kv_attn_tile_kernel<T, K, D, QC>, hipFuncAttributeMaxDynamicSharedMemorySize, smem)); });
+                t.nq = up((long)b.max_new * t.G, 64 * QC);
+                kv_attn_tile_kernel<T, K, D, QC><<<(unsigned)((long)b.n_seqs * c.n_kv_heads * t.nq * p.tile_splits), 256, smem, st>>>(a, t);
+                SS_LAUNCH_CHECK();
+            };
+            if (p.qc == 1) go(Int<1>()); else go(Int<2>());
+            join(0);
+        }
+    });
+}
+
+}  // namespace ss
