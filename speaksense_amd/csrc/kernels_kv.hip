@@ -8,6 +8,7 @@
 // p % page_size of page page_table[s][p / page_size].  Every index that comes from device memory is checked here before it is used: a page number
 // outside [0, n_pages) holds nothing (its keys are masked, reads give zeros, writes are dropped), spans of q_start outside the token rows are empty.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "gemm_common.h"
@@ -16,6 +17,12 @@
 
 namespace ss {
 namespace {
+
+// LDS of the tile kernel: pitches of a key and of a value row (16-bit elements), bytes of one stage.  The 16 key rows that a wave's lanes read 16 bytes of
+// each start on 16 different groups of 4 banks, the 8 value rows that 32 lanes read 32 bytes of on 8 different groups of 8.
+template <int D> constexpr int kKeyPitch = 2 * D + 16;
+template <int D> constexpr int kValuePitch = 2 * D + 32;
+template <int D> constexpr int kTileBuf = 64 * (kKeyPitch<D> + kValuePitch<D>) + 512;
 
 enum { K_F16 = 0, K_BF16 = 1, K_E4M3 = 2, K_I8 = 3 };   // what the cache holds
 
@@ -191,7 +198,8 @@ struct AttnArgs {
     void* out; long o_row, o_head;
     float* lse;                        // [n_tokens][heads] or null
     float* part; float2* part_ml;      // [n_tokens][heads][splits][D], [n_tokens][heads][splits]
-    float c2;                          // scale * log2(e)
+    float c2;                          // |scale| * log2(e), at least the smallest normal number: a masked -inf stays one
+    int neg;                           // scale < 0: the queries' signs are turned instead
     int G, causal, splits, split_keys; // query heads per key head; key ranges and their length (a multiple of 128)
     int all, nq;                       // tile kernel: also the sequences of at most 16 query rows; query tiles per (sequence, head)
 };
@@ -228,7 +236,7 @@ template <int KIND> __device__ __forceinline__ void codes_to_f16(unsigned w, uns
 // the 16 query rows of one column tile as B operands; returns the power of two that was taken out of this lane's row.  `dim0(s)`: first of the 8
 // dims that this lane's group contributes to k-step s
 template <typename T, typename M, int D, bool PAIRED>
-__device__ __forceinline__ float load_q(const T* q, bool ok, int g, typename Mfma<M>::V8* qf) {
+__device__ __forceinline__ float load_q(const T* q, bool ok, bool neg, int g, typename Mfma<M>::V8* qf) {
     typedef typename Mfma<T>::V8 TV8;
     TV8 x[D / 32];
 #pragma unroll
@@ -258,6 +266,9 @@ __device__ __forceinline__ float load_q(const T* q, bool ok, int g, typename Mfm
 #pragma unroll
             for (int i = 0; i < 8; i++) qf[s][i] = (M)((float)x[s][i] * m);
     }
+    if (neg)
+#pragma unroll
+        for (int s = 0; s < D / 32; s++) qf[s] = -qf[s];
     return back;
 }
 
@@ -307,30 +318,44 @@ template <typename M, int KIND, int D> struct VBlock {
 
 // Online softmax state of one column tile (a lane's query row), and the step for 32 keys
 template <typename M, bool SCALED, int D> struct Row {
-    float m = -kInf, l = 0.0f;         // l: this lane's keys only, summed over the four groups at the end
+    float m = -kInf, l = 0.0f;         // m: in log2 units; l: this lane's keys only, summed over the four groups at the end
+    float raw = 0.0f;                  // m before the factor c
+    bool far = false;                  // some row of the wave has |m| beyond 2^12: see probs
     f32x4 o[D / 16];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[i] = (f32x4){0, 0, 0, 0};
     }
-    // x[8]: scores in log2 units (-inf where masked); returns the probabilities' B operand; v[8]: value scales / sref
-    __device__ __forceinline__ typename Mfma<M>::V8 probs(const float* x, const float* v) {
-        float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__ballot(top > m + kSlack)) {
-            const float mn = fmaxf(m, rows_max(top)), ref = mn == -kInf ? 0.0f : mn;
+    // x[8]: scores (-inf where masked), c > 0: to log2 units; returns the probabilities' B operand; v[8]: value scales / sref.
+    // exp2(x c - m) is one fma and one exponential.  The fma does not round x c where m did, so every probability of the row is off by the factor
+    // 2^(x c - m at the maximum), at most 2^(|m| 2^-24), which the division by l takes out again but for what m's moves leave: below 2^-12 of it,
+    // as far as |m| <= 2^12 (the scores' own float32 steps then are as large).  Beyond that the difference is formed first.
+    __device__ __forceinline__ typename Mfma<M>::V8 probs(const float* x, float c, const float* v) {
+        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__ballot(top * c > m + kSlack)) {
+            const float rn = m == -kInf ? rows_max(top) : fmaxf(raw, rows_max(top)), mn = rn * c, ref = mn == -kInf ? 0.0f : mn;
             const float a = __builtin_amdgcn_exp2f(m - ref);
             m = mn;
+            raw = mn == -kInf ? 0.0f : rn;
+            far = __ballot(fabsf(ref) > 4096.0f) != 0;
             l *= a;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) o[i] *= a;
         }
         const float ref = m == -kInf ? 0.0f : m;
+        float e[8];
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f((x[j] - raw) * c);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c, -ref));
+        }
         typename Mfma<M>::V8 p;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float e = __builtin_amdgcn_exp2f(x[j] - ref);
-            l += e;
-            p[j] = (M)(SCALED ? e * v[j] : e);
+            l += e[j];
+            p[j] = (M)(SCALED ? e[j] * v[j] : e[j]);
         }
         return p;
     }
@@ -440,8 +465,8 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
     const int limit = !mine ? 0 : t.causal ? max(0, min(sp.pos0 + tok + 1, sp.len)) : sp.len;     // keys this lane's query row sees
     const int full = t.causal ? max(0, min(sp.pos0 + 1, sp.len)) : sp.len;                        // keys every row sees
     V8 qf[D / 32];
-    const float back = load_q<T, M, D, SCALED>((const T*)t.q + (long)row * t.q_row + (long)head * t.q_head, mine, g, qf);
-    const float c2 = t.c2 * back;
+    const float back = load_q<T, M, D, SCALED>((const T*)t.q + (long)row * t.q_row + (long)head * t.q_head, mine, t.neg, g, qf);
+    const float c2 = fmaxf(t.c2 * back, 1.17549435e-38f);
 
     const int lo = split * t.split_keys, hi = split == t.splits - 1 ? sp.len : min(sp.len, lo + t.split_keys);
     const int n = hi > lo ? (hi - lo + 31) / 32 : 0, mine_n = n > wave ? (n - wave + 3) / 4 : 0;   // tiles of the range / of this wave
@@ -481,7 +506,7 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
                 z = Mfma<M>::mma(kf, qf[d], z);
             }
 #pragma unroll
-            for (int r = 0; r < 4; r++) sc[4 * b + r] = z[r] * (SCALED ? c2 * x.ks[4 * b + r] : c2);
+            for (int r = 0; r < 4; r++) sc[4 * b + r] = SCALED ? z[r] * x.ks[4 * b + r] : z[r];
         }
         if (key0 + 32 > full || x.page[0] < 0 || x.page[1] < 0) {
 #pragma unroll
@@ -505,7 +530,7 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
 #pragma unroll
             for (int j = 0; j < 8; j++) x.vs[j] *= inv;
         }
-        const V8 p = st.probs(sc, x.vs);
+        const V8 p = st.probs(sc, c2, x.vs);
         V8 vf[N];
         x.v.frags(vf);
         st.add(vf, p);
@@ -557,16 +582,23 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
 }
 
 // ---- many query rows: a workgroup of 4 waves owns 64 QC query rows of one (sequence, key head), each wave 16 QC of them; 64-key tiles of K and V go
-// through LDS as 16 bits (8-bit codes are converted once, on the way in), the next tile's loads fly while one is computed, one barrier a tile. ----
+// through LDS as 16 bits (8-bit codes are converted once, on the way in), the next tile's loads fly while one is computed, the page numbers of the one
+// after that are on their way too; one barrier a tile.  V fragments come out of LDS by the transposing read (ds_read_b64_tr_b16: of each 16 lanes, lane i
+// names 4 columns of row i / 4 and receives 4 rows of column i), columns 16 n + (lane & 15) for MFMA n. ----
+template <typename M> __device__ __forceinline__ typename Mfma<M>::V8 read_tr(const char* p0, const char* p1) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    struct { s16x4 lo, hi; } v{__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p0), __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p1)};
+    return __builtin_bit_cast(typename Mfma<M>::V8, v);
+}
+
 template <typename T, int KIND, int D, int QC>
-__global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t) {
+__global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs t) {
     typedef typename Held<KIND>::M M;
     typedef typename Mfma<M>::V8 V8;
     constexpr bool SCALED = Held<KIND>::B == 1;
     constexpr int N = D / 16, B = Held<KIND>::B;
-    // row pitches: the 16 key rows a wave's lanes read 16 bytes of each fall on 64 different banks, and so do two value rows 4 apart
-    constexpr int KP = D * 2 + 16, VP = D == 64 ? D * 2 + 32 : D * 2 + 16;
-    constexpr int kBuf = 64 * (KP + VP) + 512;
+    constexpr int KP = kKeyPitch<D>, VP = kValuePitch<D>, kBuf = kTileBuf<D>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     int bid = blockIdx.x;
@@ -584,17 +616,21 @@ __global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t)
     if (rows <= r0 || (rows <= 16 && !t.all)) return;
 
     const int w0 = r0 + wave * (16 * QC);                  // this wave's first query row
-    int limit[QC], orow[QC], ohead[QC];
+    int limit[QC];
     V8 qf[QC][D / 32];
     float c2[QC];
+    auto row_of = [&](int i, int* head) {                  // token row and head of column tile i's row (of row 0 where there is none)
+        const int q = w0 + 16 * i + c, ok = q < rows, tok = ok ? q / t.G : 0;
+        *head = h * t.G + (ok ? q - tok * t.G : 0);
+        return sp.q0 + tok;
+    };
 #pragma unroll
     for (int i = 0; i < QC; i++) {
-        const int q = w0 + 16 * i + c, tok = q / t.G;
-        const bool ok = q < rows;
-        orow[i] = sp.q0 + (ok ? tok : 0);
-        ohead[i] = h * t.G + (ok ? q - tok * t.G : 0);
-        limit[i] = !ok ? 0 : t.causal ? max(0, min(sp.pos0 + tok + 1, sp.len)) : sp.len;
-        c2[i] = t.c2 * load_q<T, M, D, false>((const T*)t.q + (long)orow[i] * t.q_row + (long)ohead[i] * t.q_head, ok, g, qf[i]);
+        int head;
+        const int row = row_of(i, &head);
+        const bool ok = w0 + 16 * i + c < rows;
+        limit[i] = !ok ? 0 : t.causal ? max(0, min(sp.pos0 + (row - sp.q0) + 1, sp.len)) : sp.len;
+        c2[i] = fmaxf(t.c2 * load_q<T, M, D, false>((const T*)t.q + (long)row * t.q_row + (long)head * t.q_head, ok, t.neg, g, qf[i]), 1.17549435e-38f);
     }
     const int last = min(rows, r0 + 64 * QC) - 1;
     const int end = t.causal ? max(0, min(sp.pos0 + last / t.G + 1, sp.len)) : sp.len;            // keys any row of the workgroup sees
@@ -612,34 +648,47 @@ __global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t)
     constexpr int PR = D * B / 16, RP = 256 / PR, NP = 64 / RP;
     u32x4 gk[NP], gv[NP];
     float gks = 0.0f, gvs = 0.0f;      // threads 0..63: the scales of the tile's rows
+    int id[NP], sid = -1, hid = -1;    // page numbers for the next fetch: of this thread's rows, of its scale row, of 16 keys each (lanes 0..3)
+    unsigned okay = 0;                 // of the fetched tile: bit p = piece p lies on a page, bit 31 = the scales do
+    int bad = 0;                       // of the fetched tile: bit b = its keys 16 b .. 16 b + 15 lie on no page
     const int mask = (1 << a.page_shift) - 1;
-    auto fetch = [&](int i) {
+    const int* trow = a.table + (long)s * a.table_stride;
+    auto entry = [&](int key) { return key < sp.len ? trow[key >> a.page_shift] : -1; };          // key < len <= max_pages * page_size
+    auto there = [&](int page) { return page >= 0 && page < a.n_pages; };
+    auto ids = [&](int i) {
         const int key0 = lo + i * 64;
 #pragma unroll
+        for (int p = 0; p < NP; p++) id[p] = entry(key0 + tid / PR + p * RP);
+        if (SCALED && wave == 0) sid = entry(key0 + lane);
+        if (lane < 4) hid = entry(key0 + 16 * lane);
+    };
+    auto fetch = [&](int i) {          // tile i; ids(i) has run
+        const int key0 = lo + i * 64;
+        okay = 0;
+#pragma unroll
         for (int p = 0; p < NP; p++) {
-            const int key = key0 + tid / PR + p * RP;
-            const int page = key < sp.len ? page_at(a, s, key >> a.page_shift) : -1;
-            const long off = (long)max(page, 0) * a.page_bytes + (((long)h << a.page_shift) + (key & mask)) * (D * B) + (tid % PR) * 16;
+            const int key = key0 + tid / PR + p * RP, page = there(id[p]) ? id[p] : 0;
+            if (there(id[p])) okay |= 1u << p;
+            const long off = (long)page * a.page_bytes + (((long)h << a.page_shift) + (key & mask)) * (D * B) + (tid % PR) * 16;
             gk[p] = *(const u32x4*)(a.k + off);
             gv[p] = *(const u32x4*)(a.v + off);
-            if (page < 0) { gk[p] = (u32x4){0, 0, 0, 0}; gv[p] = (u32x4){0, 0, 0, 0}; }     // whatever lies there must not meet a probability of 0
         }
-        if constexpr (SCALED)
-            if (tid < 64) {
-                const int key = key0 + tid, page = key < sp.len ? page_at(a, s, key >> a.page_shift) : -1;
-                const long at = (long)max(page, 0) * a.sc_stride + ((long)h << a.page_shift) + (key & mask);
-                if constexpr (KIND == K_E4M3) {
-                    gks = __uint_as_float((unsigned)(unsigned char)a.ks[at] << 23);
-                    gvs = __uint_as_float((unsigned)(unsigned char)a.vs[at] << 23);
-                } else { gks = ((const float*)a.ks)[at]; gvs = ((const float*)a.vs)[at]; }
-                if (page < 0) { gks = 0.0f; gvs = 0.0f; }
-            }
+        if (SCALED && wave == 0) {
+            const long at = (long)(there(sid) ? sid : 0) * a.sc_stride + ((long)h << a.page_shift) + ((key0 + lane) & mask);
+            if (there(sid)) okay |= 1u << 31;
+            if constexpr (KIND == K_E4M3) {
+                gks = __uint_as_float((unsigned)(unsigned char)a.ks[at] << 23);
+                gvs = __uint_as_float((unsigned)(unsigned char)a.vs[at] << 23);
+            } else { gks = ((const float*)a.ks)[at]; gvs = ((const float*)a.vs)[at]; }
+        }
+        bad = (int)__ballot(lane < 4 && key0 + 16 * lane < sp.len && !there(hid));
     };
     auto put = [&](char* buf) {
 #pragma unroll
         for (int p = 0; p < NP; p++) {
             const int r = tid / PR + p * RP;
             char *kd = buf + r * KP, *vd = buf + 64 * KP + r * VP;
+            if (!(okay >> p & 1)) gv[p] = (u32x4){0, 0, 0, 0};     // whatever lies there must not meet a probability of 0
             if constexpr (!SCALED) {
                 *(u32x4*)(kd + (tid % PR) * 16) = gk[p];
                 *(u32x4*)(vd + (tid % PR) * 16) = gv[p];
@@ -656,27 +705,29 @@ __global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t)
                 *(u32x4*)(vd + (tid % PR) * 32 + 16) = x[1];
             }
         }
-        if constexpr (SCALED)
-            if (tid < 64) { ((float*)(buf + 64 * (KP + VP)))[tid] = gks; ((float*)(buf + 64 * (KP + VP)))[64 + tid] = gvs; }
+        if (SCALED && wave == 0) {
+            float* sc = (float*)(buf + 64 * (KP + VP));
+            sc[lane] = okay >> 31 ? gks : 0.0f;
+            sc[64 + lane] = okay >> 31 ? gvs : 0.0f;
+        }
     };
-    auto holes = [&](int key0) {       // bit b: the 16 keys from key0 + 16 b on lie on a page that is not there
-        int bad = 0;
-#pragma unroll
-        for (int b = 0; b < 4; b++) bad |= key0 + 16 * b < sp.len && page_at(a, s, (key0 + 16 * b) >> a.page_shift) < 0 ? 1 << b : 0;
-        return bad;
-    };
+    int hole = 0;                      // `bad` of the tile that is computed
     if (n > 0) {
+        ids(0);
         fetch(0);
+        hole = bad;
+        if (n > 1) ids(1);
         put(smem);
         if (n > 1) fetch(1);
+        if (n > 2) ids(2);
     }
     __syncthreads();
+    const int koff = c * KP + g * 16, voff = 64 * KP + (4 * g + (c >> 2)) * VP + (c & 3) * 8;
     for (int i = 0; i < n; i++) {
         const char* buf = smem + (i & 1) * kBuf;
         const int key0 = lo + i * 64;
         if (key0 < wend) {
-            const int bad = holes(key0);
-            const bool edge = key0 + 64 > full || bad;
+            const bool edge = key0 + 64 > full || hole;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 float vs[8], ks[8];
@@ -701,52 +752,45 @@ __global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t)
                 float x[QC][8];
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const char* kp = buf + (half * 32 + 16 * b + c) * KP + g * 16;
                     V8 kf[D / 32];
 #pragma unroll
-                    for (int d = 0; d < D / 32; d++) kf[d] = *(const V8*)(kp + d * 64);
+                    for (int d = 0; d < D / 32; d++) kf[d] = *(const V8*)(buf + koff + (half * 32 + 16 * b) * KP + d * 64);
 #pragma unroll
                     for (int j = 0; j < QC; j++) {
                         f32x4 z = {0, 0, 0, 0};
 #pragma unroll
                         for (int d = 0; d < D / 32; d++) z = Mfma<M>::mma(kf[d], qf[j][d], z);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) x[j][4 * b + r] = z[r] * (SCALED ? c2[j] * ks[4 * b + r] : c2[j]);
+                        for (int r = 0; r < 4; r++) x[j][4 * b + r] = SCALED ? z[r] * ks[4 * b + r] : z[r];
                     }
                 }
                 if (edge) {
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         const int key = key0 + half * 32 + 16 * (e >> 2) + 4 * g + (e & 3);
-                        const bool hole = bad >> (2 * half + (e >> 2)) & 1;
+                        const bool gone = hole >> (2 * half + (e >> 2)) & 1;
 #pragma unroll
                         for (int j = 0; j < QC; j++)
-                            if (hole || key >= limit[j]) x[j][e] = -kInf;
+                            if (gone || key >= limit[j]) x[j][e] = -kInf;
                     }
                 }
                 V8 p[QC];
 #pragma unroll
-                for (int j = 0; j < QC; j++) p[j] = st[j].probs(x[j], vs);
-                VBlock<M, KIND == K_BF16 ? K_BF16 : K_F16, D> vb;
+                for (int j = 0; j < QC; j++) p[j] = st[j].probs(x[j], c2[j], vs);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const char* vp = buf + 64 * KP + (half * 32 + 16 * (e >> 2) + 4 * g + (e & 3)) * VP + c * (2 * N);
-                    if constexpr (N == 4) { const u32x2 w = *(const u32x2*)vp; vb.w[e][0] = w[0]; vb.w[e][1] = w[1]; }
-                    else {
-                        const u32x4 w = *(const u32x4*)vp;
+                for (int k = 0; k < N; k++) {
+                    const char* vp = buf + voff + half * 32 * VP + k * 32;
+                    const V8 vf = read_tr<M>(vp, vp + 16 * VP);
 #pragma unroll
-                        for (int q = 0; q < 4; q++) vb.w[e][q] = w[q];
-                    }
+                    for (int j = 0; j < QC; j++) st[j].o[k] = Mfma<M>::mma(vf, p[j], st[j].o[k]);
                 }
-                V8 vf[N];
-                vb.frags(vf);
-#pragma unroll
-                for (int j = 0; j < QC; j++) st[j].add(vf, p[j]);
             }
         }
         if (i + 1 < n) {
+            hole = bad;
             put(smem + ((i + 1) & 1) * kBuf);              // last read before the barrier that ended tile i - 1
             if (i + 2 < n) fetch(i + 2);
+            if (i + 3 < n) ids(i + 3);
         }
         __syncthreads();
     }
@@ -754,25 +798,29 @@ __global__ __launch_bounds__(256) void kv_attn_tile_kernel(KvArgs a, AttnArgs t)
     for (int j = 0; j < QC; j++) {
         const float L = rows_sum(st[j].l), mm = st[j].m;
         if (w0 + 16 * j + c >= rows) continue;
-        const long at = (long)orow[j] * (a.H * t.G) + ohead[j];
+        int head;
+        const int row = row_of(j, &head);
+        const long at = (long)row * (a.H * t.G) + head;
         const float u = SCALED ? sr.ref : 1.0f;
         if (t.splits == 1) {
             const float inv = (L > 0.0f ? 1.0f / L : L) * u;
-            T* o = (T*)t.out + (long)orow[j] * t.o_row + (long)ohead[j] * t.o_head;
+            T* o = (T*)t.out + (long)row * t.o_row + (long)head * t.o_head;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float y[N];
+            for (int k = 0; k < N; k++) {
+                float y[4];
 #pragma unroll
-                for (int k = 0; k < N; k++) y[k] = L == 0.0f ? 0.0f : st[j].o[k][r] * inv;
-                store_cols<T, N>(o + N * (4 * g + r), y);
+                for (int r = 0; r < 4; r++) y[r] = L == 0.0f ? 0.0f : st[j].o[k][r] * inv;
+                store_cols<T, 4>(o + 16 * k + 4 * g, y);
             }
             if (t.lse && g == 0) t.lse[at] = L > 0.0f ? (mm + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
         } else {
             float* o = t.part + (at * t.splits + split) * D;
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int k = 0; k < N; k++) o[N * (4 * g + r) + k] = L == 0.0f ? 0.0f : st[j].o[k][r] * u;
+            for (int k = 0; k < N; k++) {
+                f32x4 y = {0, 0, 0, 0};
+                if (L != 0.0f) y = st[j].o[k] * u;
+                *(f32x4*)(o + 16 * k + 4 * g) = y;
+            }
             if (g == 0) t.part_ml[at * t.splits + split] = make_float2(mm, L);
         }
     }
@@ -887,7 +935,7 @@ void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv
     AttnArgs t{};
     t.q = q.p; t.q_row = q.row_stride; t.q_head = q.head_stride;
     t.out = out.p; t.o_row = out.row_stride; t.o_head = out.head_stride;
-    t.lse = lse; t.c2 = scale * 1.44269504088896340736f; t.G = n_heads / c.n_kv_heads; t.causal = causal;
+    t.lse = lse; t.c2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f); t.neg = scale < 0.0f; t.G = n_heads / c.n_kv_heads; t.causal = causal;
     t.all = p.tile && !p.few;
     by_type(c, [&](auto tt, auto kind, auto dim) {
         typedef decltype(tt) T;
@@ -911,7 +959,7 @@ void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv
         if (p.tile) {
             part(p.tile_splits, p.tile_keys);
             auto go = [&](auto qc) {
-                constexpr int QC = qc.value, smem = 2 * (64 * (D * 2 + 16 + (D == 64 ? D * 2 + 32 : D * 2 + 16)) + 512);
+                constexpr int QC = qc.value, smem = 2 * kTileBuf<D>;
                 static std::atomic<uint64_t> once{0};
                 once_per_device(once, [&] { SS_HIP(hipFuncSetAttribute((const void*)kv_attn_tile_kernel<T, K, D, QC>, hipFuncAttributeMaxDynamicSharedMemorySize, smem)); });
                 t.nq = up((long)b.max_new * t.G, 64 * QC);
