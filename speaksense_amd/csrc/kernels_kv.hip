@@ -22,7 +22,7 @@ namespace {
 // each start on 16 different groups of 4 banks, the 8 value rows that 32 lanes read 32 bytes of on 8 different groups of 8.
 template <int D> constexpr int kKeyPitch = 2 * D + 16;
 template <int D> constexpr int kValuePitch = 2 * D + 32;
-template <int D> constexpr int kTileBuf = 64 * (kKeyPitch<D> + kValuePitch<D>) + 512;
+template <int D> constexpr int kTileBuf = 64 * (kKeyPitch<D> + kValuePitch<D>) + 528;   // + 64 key scales, 64 relative value scales, sref, its move
 
 enum { K_F16 = 0, K_BF16 = 1, K_E4M3 = 2, K_I8 = 3 };   // what the cache holds
 
@@ -320,44 +320,19 @@ template <typename M, int KIND, int D> struct VBlock {
 template <typename M, bool SCALED, int D> struct Row {
     float m = -kInf, l = 0.0f;         // m: in log2 units; l: this lane's keys only, summed over the four groups at the end
     float raw = 0.0f;                  // m before the factor c
-    bool far = false;                  // some row of the wave has |m| beyond 2^12: see probs
     f32x4 o[D / 16];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[i] = (f32x4){0, 0, 0, 0};
     }
-    // x[8]: scores (-inf where masked), c > 0: to log2 units; returns the probabilities' B operand; v[8]: value scales / sref.
-    // exp2(x c - m) is one fma and one exponential.  The fma does not round x c where m did, so every probability of the row is off by the factor
-    // 2^(x c - m at the maximum), at most 2^(|m| 2^-24), which the division by l takes out again but for what m's moves leave: below 2^-12 of it,
-    // as far as |m| <= 2^12 (the scores' own float32 steps then are as large).  Beyond that the difference is formed first.
-    __device__ __forceinline__ typename Mfma<M>::V8 probs(const float* x, float c, const float* v) {
-        const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__ballot(top * c > m + kSlack)) {
-            const float rn = m == -kInf ? rows_max(top) : fmaxf(raw, rows_max(top)), mn = rn * c, ref = mn == -kInf ? 0.0f : mn;
-            const float a = __builtin_amdgcn_exp2f(m - ref);
-            m = mn;
-            raw = mn == -kInf ? 0.0f : rn;
-            far = __ballot(fabsf(ref) > 4096.0f) != 0;
-            l *= a;
+    __device__ __forceinline__ void move(float top, float c) {          // m up to the largest score so far, what was summed along with it
+        const float rn = m == -kInf ? rows_max(top) : fmaxf(raw, rows_max(top)), mn = rn * c, ref = mn == -kInf ? 0.0f : mn;
+        const float a = __builtin_amdgcn_exp2f(m - ref);
+        m = mn;
+        raw = mn == -kInf ? 0.0f : rn;
+        l *= a;
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) o[i] *= a;
-        }
-        const float ref = m == -kInf ? 0.0f : m;
-        float e[8];
-        if (__builtin_expect(far, 0)) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f((x[j] - raw) * c);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(x[j], c, -ref));
-        }
-        typename Mfma<M>::V8 p;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            l += e[j];
-            p[j] = (M)(SCALED ? e[j] * v[j] : e[j]);
-        }
-        return p;
+        for (int i = 0; i < D / 16; i++) o[i] *= a;
     }
     __device__ __forceinline__ void add(const typename Mfma<M>::V8* vf, typename Mfma<M>::V8 p) {
 #pragma unroll
@@ -365,12 +340,53 @@ template <typename M, bool SCALED, int D> struct Row {
     }
 };
 
+// Scores x[QC][8] of 32 keys (-inf where masked; c > 0 brings them to log2 units) -> the probabilities' B operands; v[8]: value scales / sref.
+// exp2(x c - m) is one fma and one exponential.  The fma does not round x c where m did, so every probability of the row is off by the factor
+// 2^(x c - m at the maximum), at most 2^(|m| 2^-24), which the division by l takes out again but for what m's moves leave: below 2^-12 of it as far
+// as |m| <= 2^12 (the scores' own float32 steps then are as large).  Beyond that (far, the same for the whole wave) the difference is formed first.
+template <int QC, typename M, bool SCALED, int D>
+__device__ __forceinline__ void softmax_step(Row<M, SCALED, D>* st, bool& far, float (*x)[8], const float* c, const float* v, typename Mfma<M>::V8* p) {
+    float top[QC], ref[QC];
+    bool moved = false;
+#pragma unroll
+    for (int j = 0; j < QC; j++) {
+        top[j] = fmaxf(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])), fmaxf(fmaxf(x[j][4], x[j][5]), fmaxf(x[j][6], x[j][7])));
+        moved |= top[j] * c[j] > st[j].m + kSlack;
+        ref[j] = st[j].m == -kInf ? 0.0f : st[j].m;
+    }
+    if (__ballot(moved) || far) {
+        asm volatile("");              // a branch, not selects
+        bool f = false;
+#pragma unroll
+        for (int j = 0; j < QC; j++) {
+            st[j].move(top[j], c[j]);
+            ref[j] = st[j].m == -kInf ? 0.0f : st[j].m;
+            f |= fabsf(ref[j]) > 4096.0f;
+        }
+        far = __ballot(f) != 0;
+        if (far)
+#pragma unroll
+            for (int j = 0; j < QC; j++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[j][e] -= st[j].raw;
+                ref[j] = 0.0f;
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < QC; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(x[j][e], c[j], -ref[j]));
+            st[j].l += w;
+            p[j][e] = (M)(SCALED ? w * v[e] : w);
+        }
+}
+
 // the running power of two near the largest value scale; one per wave
 struct ScaleRef {
     float ref = 0.0f;
-    // returns what O has to be multiplied by (1 when nothing moved)
-    __device__ __forceinline__ bool moves(const float* v, float* by) {
-        const float top = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    // of the scales of a tile, `top` the lane's largest: did it move, and what O has to be multiplied by then
+    __device__ __forceinline__ bool moves(float top, float* by) {
         if (!__ballot(top > ref * 64.0f)) return false;
         const float n = __uint_as_float(__float_as_uint(fmaxf(wave_max(top), ref)) & 0x7f800000u);
         *by = n > 0.0f ? ref / n : 0.0f;
@@ -472,6 +488,7 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
     const int n = hi > lo ? (hi - lo + 31) / 32 : 0, mine_n = n > wave ? (n - wave + 3) / 4 : 0;   // tiles of the range / of this wave
     Row<M, SCALED, D> st;
     st.clear();
+    bool far = false;
     ScaleRef sr;
 
     int ids[2] = {-1, -1};             // lane i: the pages of this wave's tile i of the current 64
@@ -523,14 +540,16 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
         }
         if constexpr (SCALED) {
             float by;
-            if (sr.moves(x.vs, &by))
+            const float* v = x.vs;
+            if (sr.moves(fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]))), &by))
 #pragma unroll
                 for (int k = 0; k < N; k++) st.o[k] *= by;
             const float inv = sr.inv();
 #pragma unroll
             for (int j = 0; j < 8; j++) x.vs[j] *= inv;
         }
-        const V8 p = st.probs(sc, c2, x.vs);
+        V8 p;
+        softmax_step<1>(&st, far, &sc, &c2, x.vs, &p);
         V8 vf[N];
         x.v.frags(vf);
         st.add(vf, p);
@@ -705,10 +724,14 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
                 *(u32x4*)(vd + (tid % PR) * 32 + 16) = x[1];
             }
         }
-        if (SCALED && wave == 0) {
+        if (SCALED && wave == 0) {     // the first wave keeps sref and hands out what follows from it
             float* sc = (float*)(buf + 64 * (KP + VP));
+            const float v = okay >> 31 ? gvs : 0.0f;
+            float by = 1.0f;
+            sr.moves(v, &by);
             sc[lane] = okay >> 31 ? gks : 0.0f;
-            sc[64 + lane] = okay >> 31 ? gvs : 0.0f;
+            sc[64 + lane] = v * sr.inv();
+            if (lane == 0) { sc[128] = sr.ref; sc[129] = by; }
         }
     };
     int hole = 0;                      // `bad` of the tile that is computed
@@ -723,69 +746,72 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     }
     __syncthreads();
     const int koff = c * KP + g * 16, voff = 64 * KP + (4 * g + (c >> 2)) * VP + (c & 3) * 8;
+    bool far = false;
+    float ref = 1.0f;                  // sref of what this wave has summed
+    auto compute = [&](bool edge, const char* buf, int key0) {      // edge: some key of the tile is masked for some row of the wave
+        const float* sc = (const float*)(buf + 64 * (KP + VP));
+        if constexpr (SCALED) {
+            ref = sc[128];
+            const float by = sc[129];
+            if (__builtin_amdgcn_readfirstlane(__float_as_int(by)) != __float_as_int(1.0f))
+#pragma unroll
+                for (int j = 0; j < QC; j++)
+#pragma unroll
+                    for (int k = 0; k < N; k++) st[j].o[k] *= by;
+        }
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            float vs[8], x[QC][8];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                V8 kf[D / 32];
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) kf[d] = *(const V8*)(buf + koff + (half * 32 + 16 * b) * KP + d * 64);
+                f32x4 ks;
+                if constexpr (SCALED) {
+                    ks = *(const f32x4*)(sc + half * 32 + 16 * b + 4 * g);
+                    const f32x4 y = *(const f32x4*)(sc + 64 + half * 32 + 16 * b + 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) vs[4 * b + r] = y[r];
+                }
+                f32x4 z[QC];
+#pragma unroll
+                for (int j = 0; j < QC; j++) z[j] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < D / 32; d++)
+#pragma unroll
+                    for (int j = 0; j < QC; j++) z[j] = Mfma<M>::mma(kf[d], qf[j][d], z[j]);
+#pragma unroll
+                for (int j = 0; j < QC; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[j][4 * b + r] = SCALED ? z[j][r] * ks[r] : z[j][r];
+            }
+            if (edge) {
+                asm volatile("");      // a branch: the selects are not worth their time on the tiles that need none
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + half * 32 + 16 * (e >> 2) + 4 * g + (e & 3);
+                    const bool gone = hole >> (2 * half + (e >> 2)) & 1;
+#pragma unroll
+                    for (int j = 0; j < QC; j++)
+                        if (gone || key >= limit[j]) x[j][e] = -kInf;
+                }
+            }
+            V8 p[QC];
+            softmax_step<QC>(st, far, x, c2, vs, p);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const char* vp = buf + voff + half * 32 * VP + k * 32;
+                const V8 vf = read_tr<M>(vp, vp + 16 * VP);
+#pragma unroll
+                for (int j = 0; j < QC; j++) st[j].o[k] = Mfma<M>::mma(vf, p[j], st[j].o[k]);
+            }
+        }
+    };
     for (int i = 0; i < n; i++) {
         const char* buf = smem + (i & 1) * kBuf;
         const int key0 = lo + i * 64;
-        if (key0 < wend) {
-            const bool edge = key0 + 64 > full || hole;
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float vs[8], ks[8];
-                if constexpr (SCALED) {
-                    const float* sc = (const float*)(buf + 64 * (KP + VP));
-#pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const f32x4 x = *(const f32x4*)(sc + half * 32 + 16 * b + 4 * g), y = *(const f32x4*)(sc + 64 + half * 32 + 16 * b + 4 * g);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) { ks[4 * b + r] = x[r]; vs[4 * b + r] = y[r]; }
-                    }
-                    float by;
-                    if (sr.moves(vs, &by))
-#pragma unroll
-                        for (int j = 0; j < QC; j++)
-#pragma unroll
-                            for (int k = 0; k < N; k++) st[j].o[k] *= by;
-                    const float inv = sr.inv();
-#pragma unroll
-                    for (int j = 0; j < 8; j++) vs[j] *= inv;
-                }
-                float x[QC][8];
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    V8 kf[D / 32];
-#pragma unroll
-                    for (int d = 0; d < D / 32; d++) kf[d] = *(const V8*)(buf + koff + (half * 32 + 16 * b) * KP + d * 64);
-#pragma unroll
-                    for (int j = 0; j < QC; j++) {
-                        f32x4 z = {0, 0, 0, 0};
-#pragma unroll
-                        for (int d = 0; d < D / 32; d++) z = Mfma<M>::mma(kf[d], qf[j][d], z);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) x[j][4 * b + r] = SCALED ? z[r] * ks[4 * b + r] : z[r];
-                    }
-                }
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int key = key0 + half * 32 + 16 * (e >> 2) + 4 * g + (e & 3);
-                        const bool gone = hole >> (2 * half + (e >> 2)) & 1;
-#pragma unroll
-                        for (int j = 0; j < QC; j++)
-                            if (gone || key >= limit[j]) x[j][e] = -kInf;
-                    }
-                }
-                V8 p[QC];
-#pragma unroll
-                for (int j = 0; j < QC; j++) p[j] = st[j].probs(x[j], c2[j], vs);
-#pragma unroll
-                for (int k = 0; k < N; k++) {
-                    const char* vp = buf + voff + half * 32 * VP + k * 32;
-                    const V8 vf = read_tr<M>(vp, vp + 16 * VP);
-#pragma unroll
-                    for (int j = 0; j < QC; j++) st[j].o[k] = Mfma<M>::mma(vf, p[j], st[j].o[k]);
-                }
-            }
-        }
+        if (key0 < wend) compute(key0 + 64 > full || hole, buf, key0);
         if (i + 1 < n) {
             hole = bad;
             put(smem + ((i + 1) & 1) * kBuf);              // last read before the barrier that ended tile i - 1
@@ -801,7 +827,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
         int head;
         const int row = row_of(j, &head);
         const long at = (long)row * (a.H * t.G) + head;
-        const float u = SCALED ? sr.ref : 1.0f;
+        const float u = SCALED ? ref : 1.0f;
         if (t.splits == 1) {
             const float inv = (L > 0.0f ? 1.0f / L : L) * u;
             T* o = (T*)t.out + (long)row * t.o_row + (long)head * t.o_head;
