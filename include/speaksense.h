@@ -371,8 +371,8 @@ typedef struct ss_kv_cache {      /* one layer */
     void* v;
     void* k_scale;                /* [n_pages][n_kv_heads][page_size], NULL for SS_KV_SAME: */
     void* v_scale;                /*   SS_KV_E4M3 uint8 E8M0 exponents, SS_KV_INT8 float32; 16-byte aligned */
-    int64_t page_stride;          /* elements from one page of k (and v) to the next: >= n_kv_heads * page_size * head_dim, a multiple of 16 */
-    int64_t scale_stride;         /* elements from one page of the scales to the next: >= n_kv_heads * page_size, a multiple of 16 */
+    int64_t page_stride;          /* elements from one page of k (and v) to the next: >= n_kv_heads * page_size * head_dim, a multiple of 16, < 2^31 */
+    int64_t scale_stride;         /* elements from one page of the scales to the next: >= n_kv_heads * page_size, a multiple of 16, < 2^31 */
     int32_t n_pages;
     int32_t page_size;            /* a power of two from 16 to 256 */
     int32_t n_kv_heads;

@@ -557,11 +557,11 @@ const char* bad_cache(const ss_kv_cache& c) {
     if (c.page_size < 16 || c.page_size > 256 || (c.page_size & (c.page_size - 1))) return "page_size must be a power of two from 16 to 256";
     if (c.n_pages <= 0 || c.n_kv_heads <= 0 || c.n_kv_heads > 4096) return "n_pages and n_kv_heads must be positive (at most 4096 heads)";
     const int64_t rows = (int64_t)c.n_kv_heads * c.page_size;
-    if (c.page_stride < rows * c.head_dim || c.page_stride % 16 || c.page_stride > (int64_t)1 << 40) return "page_stride must hold a page and be a multiple of 16";
+    if (c.page_stride < rows * c.head_dim || c.page_stride % 16 || c.page_stride >= (int64_t)1 << 31) return "page_stride must hold a page, be a multiple of 16 and less than 2^31";
     if (!c.k || !c.v || !aligned(c.k, 16) || !aligned(c.v, 16)) return "k and v must be 16-byte aligned device pointers";
     if (c.kind != SS_KV_SAME) {
         if (!c.k_scale || !c.v_scale || !aligned(c.k_scale, 16) || !aligned(c.v_scale, 16)) return "an 8-bit cache needs 16-byte aligned k_scale and v_scale";
-        if (c.scale_stride < rows || c.scale_stride % 16 || c.scale_stride > (int64_t)1 << 40) return "scale_stride must hold a page's rows and be a multiple of 16";
+        if (c.scale_stride < rows || c.scale_stride % 16 || c.scale_stride >= (int64_t)1 << 31) return "scale_stride must hold a page's rows, be a multiple of 16 and less than 2^31";
     }
     return nullptr;
 }

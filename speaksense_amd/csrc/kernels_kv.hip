@@ -28,11 +28,14 @@ enum { K_F16 = 0, K_BF16 = 1, K_E4M3 = 2, K_I8 = 3 };   // what the cache holds
 
 struct KvArgs {
     char *k, *v, *ks, *vs;
-    long page_bytes, sc_stride;          // between pages: bytes of codes, elements of scales
+    unsigned page_bytes, sc_stride;      // between pages: bytes of codes, elements of scales (the host has checked that they fit)
     const int *table, *q_start, *kv_len;
     long table_stride;
     int n_pages, page_shift, H, max_pages, n_seqs, n_tokens;
 };
+
+// a + page * pitch: one multiply-add of 32 x 32 + 64 bits
+__device__ __forceinline__ char* page_ptr(char* a, int page, unsigned pitch) { return a + (unsigned long)(unsigned)page * pitch; }
 
 struct Span { int q0, n_new, len, pos0; };   // first token row, new tokens, positions held, position of the first new token
 __device__ __forceinline__ Span seq_span(const KvArgs& a, int s) {
@@ -97,7 +100,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, const T* __res
     const T* src = is_v ? vn + (long)t * v_row + (long)h * v_head : kn + (long)t * k_row + (long)h * k_head;
     const V8 x = *(const V8*)(src + c * 8);
     const long slot = ((long)h << a.page_shift) + (pos & ((1 << a.page_shift) - 1));   // row inside the page
-    char* dst = (is_v ? a.v : a.k) + (long)page * a.page_bytes;
+    char* dst = page_ptr(is_v ? a.v : a.k, page, a.page_bytes);
     if constexpr (KIND == K_F16 || KIND == K_BF16) {
         *(V8*)(dst + (slot * D + c * 8) * 2) = x;
     } else {
@@ -108,7 +111,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, const T* __res
         top = lanes_umax<LPR>(top);
         uint2 code;
         char* sc = is_v ? a.vs : a.ks;
-        const long at = (long)page * a.sc_stride + slot;
+        const long at = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
         if constexpr (KIND == K_E4M3) {
             const int e = e8m0_for_amax(__uint_as_float(top));
             const float m = pow2_neg_of_e8m0(e);
@@ -150,13 +153,13 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, T* __restrict__ 
     for (int i = 0; i < 8; i++) x[i] = (T)0.0f;
     if (page >= 0) {
         const long slot = ((long)h << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-        const char* src = (is_v ? a.v : a.k) + (long)page * a.page_bytes;
+        const char* src = page_ptr(is_v ? a.v : a.k, page, a.page_bytes);
         if constexpr (KIND == K_F16 || KIND == K_BF16) {
             x = *(const V8*)(src + (slot * D + c * 8) * 2);
         } else {
             const uint2 code = *(const uint2*)(src + slot * D + c * 8);
             const char* sc = is_v ? a.vs : a.ks;
-            const long at = (long)page * a.sc_stride + slot;
+            const long at = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
             float f[8], m;
             if constexpr (KIND == K_E4M3) {
                 m = __uint_as_float((unsigned)(unsigned char)sc[at] << 23);
@@ -344,13 +347,15 @@ template <typename M, bool SCALED, int D> struct Row {
 // exp2(x c - m) is one fma and one exponential.  The fma does not round x c where m did, so every probability of the row is off by the factor
 // 2^(x c - m at the maximum), at most 2^(|m| 2^-24), which the division by l takes out again but for what m's moves leave: below 2^-12 of it as far
 // as |m| <= 2^12 (the scores' own float32 steps then are as large).  Beyond that (far, the same for the whole wave) the difference is formed first.
-template <int QC, typename M, bool SCALED, int D>
-__device__ __forceinline__ void softmax_step(Row<M, SCALED, D>* st, bool& far, float (*x)[8], const float* c, const float* v, typename Mfma<M>::V8* p) {
-    float top[QC], ref[QC];
+template <int QC, int NE, typename M, bool SCALED, int D>
+__device__ __forceinline__ void softmax_ref(Row<M, SCALED, D>* st, bool& far, float (*x)[NE], const float* c, float* ref) {
+    float top[QC];
     bool moved = false;
 #pragma unroll
     for (int j = 0; j < QC; j++) {
-        top[j] = fmaxf(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])), fmaxf(fmaxf(x[j][4], x[j][5]), fmaxf(x[j][6], x[j][7])));
+        top[j] = x[j][0];
+#pragma unroll
+        for (int e = 1; e < NE; e++) top[j] = fmaxf(top[j], x[j][e]);
         moved |= top[j] * c[j] > st[j].m + kSlack;
         ref[j] = st[j].m == -kInf ? 0.0f : st[j].m;
     }
@@ -368,18 +373,22 @@ __device__ __forceinline__ void softmax_step(Row<M, SCALED, D>* st, bool& far, f
 #pragma unroll
             for (int j = 0; j < QC; j++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[j][e] -= st[j].raw;
+                for (int e = 0; e < NE; e++) x[j][e] -= st[j].raw;
                 ref[j] = 0.0f;
             }
     }
+}
+// 8 scores of a lane -> its B operand
+template <typename M, bool SCALED, int D>
+__device__ __forceinline__ typename Mfma<M>::V8 probs(Row<M, SCALED, D>& st, const float* x, float c, float ref, const float* v) {
+    typename Mfma<M>::V8 p;
 #pragma unroll
-    for (int j = 0; j < QC; j++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float w = __builtin_amdgcn_exp2f(fmaf(x[j][e], c[j], -ref[j]));
-            st[j].l += w;
-            p[j][e] = (M)(SCALED ? w * v[e] : w);
-        }
+    for (int e = 0; e < 8; e++) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(x[e], c, -ref));
+        st.l += w;
+        p[e] = (M)(SCALED ? w * v[e] : w);
+    }
+    return p;
 }
 
 // the running power of two near the largest value scale; one per wave
@@ -429,8 +438,8 @@ template <int KIND, int D> struct KvTile {
         for (int b = 0; b < 2; b++) {
             const int p = max(page[b], 0), r0 = (key0 + 16 * b) & mask;     // 16 keys share a page
             const long row = ((long)h << a.page_shift) + r0;
-            const char* kp = a.k + (long)p * a.page_bytes + row * (D * B);
-            const char* vp = a.v + (long)p * a.page_bytes + row * (D * B);
+            const char* kp = page_ptr(a.k, p, a.page_bytes) + row * (D * B);
+            const char* vp = page_ptr(a.v, p, a.page_bytes) + row * (D * B);
 #pragma unroll
             for (int i = 0; i < KN; i++) k[b][i] = *(const u32x4*)(kp + m * (D * B) + 64 * i + 16 * g);
             constexpr int DW = VBlock<typename Held<KIND>::M, KIND, D>::DW;
@@ -445,7 +454,7 @@ template <int KIND, int D> struct KvTile {
                     for (int i = 0; i < 4; i++) v.w[4 * b + r][i] = t[i];
                 }
             }
-            const long at = (long)p * a.sc_stride + row + 4 * g;
+            const long at = (long)((unsigned long)(unsigned)p * a.sc_stride) + row + 4 * g;
             if constexpr (KIND == K_E4M3) {
                 const unsigned x = *(const unsigned*)(a.ks + at), y = *(const unsigned*)(a.vs + at);
 #pragma unroll
@@ -548,8 +557,9 @@ __global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) 
 #pragma unroll
             for (int j = 0; j < 8; j++) x.vs[j] *= inv;
         }
-        V8 p;
-        softmax_step<1>(&st, far, &sc, &c2, x.vs, &p);
+        float m;
+        softmax_ref<1, 8>(&st, far, &sc, &c2, &m);
+        const V8 p = probs(st, sc, c2, m, x.vs);
         V8 vf[N];
         x.v.frags(vf);
         st.add(vf, p);
@@ -688,12 +698,12 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
         for (int p = 0; p < NP; p++) {
             const int key = key0 + tid / PR + p * RP, page = there(id[p]) ? id[p] : 0;
             if (there(id[p])) okay |= 1u << p;
-            const long off = (long)page * a.page_bytes + (((long)h << a.page_shift) + (key & mask)) * (D * B) + (tid % PR) * 16;
+            const long off = (long)((unsigned long)(unsigned)page * a.page_bytes) + (((long)h << a.page_shift) + (key & mask)) * (D * B) + (tid % PR) * 16;
             gk[p] = *(const u32x4*)(a.k + off);
             gv[p] = *(const u32x4*)(a.v + off);
         }
         if (SCALED && wave == 0) {
-            const long at = (long)(there(sid) ? sid : 0) * a.sc_stride + ((long)h << a.page_shift) + ((key0 + lane) & mask);
+            const long at = (long)((unsigned long)(unsigned)(there(sid) ? sid : 0) * a.sc_stride) + ((long)h << a.page_shift) + ((key0 + lane) & mask);
             if (there(sid)) okay |= 1u << 31;
             if constexpr (KIND == K_E4M3) {
                 gks = __uint_as_float((unsigned)(unsigned char)a.ks[at] << 23);
@@ -735,16 +745,6 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
         }
     };
     int hole = 0;                      // `bad` of the tile that is computed
-    if (n > 0) {
-        ids(0);
-        fetch(0);
-        hole = bad;
-        if (n > 1) ids(1);
-        put(smem);
-        if (n > 1) fetch(1);
-        if (n > 2) ids(2);
-    }
-    __syncthreads();
     const int koff = c * KP + g * 16, voff = 64 * KP + (4 * g + (c >> 2)) * VP + (c & 3) * 8;
     bool far = false;
     float ref = 1.0f;                  // sref of what this wave has summed
@@ -759,66 +759,101 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
 #pragma unroll
                     for (int k = 0; k < N; k++) st[j].o[k] *= by;
         }
+        // scores: the next 16 keys' fragments are on their way out of LDS while these are multiplied
+        float x[QC][16];
+        V8 kf[2][D / 32];
+        auto read_k = [&](int b) {
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            float vs[8], x[QC][8];
+            for (int d = 0; d < D / 32; d++) kf[b & 1][d] = *(const V8*)(buf + koff + 16 * b * KP + d * 64);
+        };
+        read_k(0);
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                V8 kf[D / 32];
+        for (int b = 0; b < 4; b++) {
+            f32x4 z[QC], ks;
+            if constexpr (SCALED) ks = *(const f32x4*)(sc + 16 * b + 4 * g);
+            if (b < 3) read_k(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int d = 0; d < D / 32; d++) kf[d] = *(const V8*)(buf + koff + (half * 32 + 16 * b) * KP + d * 64);
-                f32x4 ks;
-                if constexpr (SCALED) {
-                    ks = *(const f32x4*)(sc + half * 32 + 16 * b + 4 * g);
-                    const f32x4 y = *(const f32x4*)(sc + 64 + half * 32 + 16 * b + 4 * g);
+            for (int j = 0; j < QC; j++) z[j] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-                    for (int r = 0; r < 4; r++) vs[4 * b + r] = y[r];
-                }
-                f32x4 z[QC];
+            for (int d = 0; d < D / 32; d++)
 #pragma unroll
-                for (int j = 0; j < QC; j++) z[j] = (f32x4){0, 0, 0, 0};
+                for (int j = 0; j < QC; j++) z[j] = Mfma<M>::mma(kf[b & 1][d], qf[j][d], z[j]);
 #pragma unroll
-                for (int d = 0; d < D / 32; d++)
+            for (int j = 0; j < QC; j++)
 #pragma unroll
-                    for (int j = 0; j < QC; j++) z[j] = Mfma<M>::mma(kf[d], qf[j][d], z[j]);
+                for (int r = 0; r < 4; r++) x[j][4 * b + r] = SCALED ? z[j][r] * ks[r] : z[j][r];
+        }
+        // values: groups of 4 column tiles of one half; a group's fragments are read while the one before is multiplied
+        constexpr int NG = N / 4;
+        V8 vf[2][4];
+        auto read_v = [&](int grp) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const char* vp = buf + voff + grp / NG * 32 * VP + (grp % NG * 4 + k) * 32;
+                vf[grp & 1][k] = read_tr<M>(vp, vp + 16 * VP);
+            }
+        };
+        read_v(0);
+        if (edge) {
+            asm volatile("");          // a branch: the selects are not worth their time on the tiles that need none
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int key = key0 + 16 * (e >> 2) + 4 * g + (e & 3);
+                const bool gone = hole >> (e >> 2) & 1;
 #pragma unroll
                 for (int j = 0; j < QC; j++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[j][4 * b + r] = SCALED ? z[j][r] * ks[r] : z[j][r];
+                    if (gone || key >= limit[j]) x[j][e] = -kInf;
             }
-            if (edge) {
-                asm volatile("");      // a branch: the selects are not worth their time on the tiles that need none
+        }
+        float m[QC];
+        softmax_ref<QC, 16>(st, far, x, c2, m);
+        float vs[2][8];
+        if constexpr (SCALED)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int key = key0 + half * 32 + 16 * (e >> 2) + 4 * g + (e & 3);
-                    const bool gone = hole >> (2 * half + (e >> 2)) & 1;
+            for (int b = 0; b < 4; b++) {
+                const f32x4 y = *(const f32x4*)(sc + 64 + 16 * b + 4 * g);
 #pragma unroll
-                    for (int j = 0; j < QC; j++)
-                        if (gone || key >= limit[j]) x[j][e] = -kInf;
+                for (int r = 0; r < 4; r++) vs[b >> 1][4 * (b & 1) + r] = y[r];
+            }
+        V8 p[2][QC];
+#pragma unroll
+        for (int j = 0; j < QC; j++) p[0][j] = probs(st[j], x[j], c2[j], m[j], vs[0]);
+#pragma unroll
+        for (int grp = 0; grp < 2 * NG; grp++) {
+            if (grp + 1 < 2 * NG) read_v(grp + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (grp < NG)              // the second half's exponentials between the first half's products
+#pragma unroll
+                for (int j = grp * QC / NG; j < (grp + 1) * QC / NG; j++) p[1][j] = probs(st[j], x[j] + 8, c2[j], m[j], vs[1]);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int j = 0; j < QC; j++) {
+                    f32x4& o = st[j].o[grp % NG * 4 + k];
+                    o = Mfma<M>::mma(vf[grp & 1][k], p[grp / NG][j], o);
                 }
-            }
-            V8 p[QC];
-            softmax_step<QC>(st, far, x, c2, vs, p);
-#pragma unroll
-            for (int k = 0; k < N; k++) {
-                const char* vp = buf + voff + half * 32 * VP + k * 32;
-                const V8 vf = read_tr<M>(vp, vp + 16 * VP);
-#pragma unroll
-                for (int j = 0; j < QC; j++) st[j].o[k] = Mfma<M>::mma(vf, p[j], st[j].o[k]);
-            }
         }
     };
-    for (int i = 0; i < n; i++) {
-        const char* buf = smem + (i & 1) * kBuf;
-        const int key0 = lo + i * 64;
-        if (key0 < wend) compute(key0 + 64 > full || hole, buf, key0);
-        if (i + 1 < n) {
-            hole = bad;
-            put(smem + ((i + 1) & 1) * kBuf);              // last read before the barrier that ended tile i - 1
-            if (i + 2 < n) fetch(i + 2);
-            if (i + 3 < n) ids(i + 3);
-        }
+    if (n > 0) {                       // one block from here to the end of the loop: nothing older than its own loads is in flight where it begins
+        ids(0);
+        fetch(0);
+        hole = bad;
+        if (n > 1) ids(1);
+        put(smem);
+        if (n > 1) fetch(1);
+        if (n > 2) ids(2);
         __syncthreads();
+        for (int i = 0;;) {
+            const int key0 = lo + i * 64;
+            if (key0 < wend) compute(key0 + 64 > full || hole, smem + (i & 1) * kBuf, key0);
+            if (++i >= n) break;
+            hole = bad;
+            put(smem + (i & 1) * kBuf);                    // last read before the barrier that ended tile i - 2
+            if (i + 1 < n) fetch(i + 1);
+            if (i + 2 < n) ids(i + 2);
+            __syncthreads();
+        }
     }
 #pragma unroll
     for (int j = 0; j < QC; j++) {
@@ -888,8 +923,8 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t,
 KvArgs kv_args(const ss_kv_cache& c, const ss_kv_batch& b) {
     KvArgs a{};
     a.k = (char*)c.k; a.v = (char*)c.v; a.ks = (char*)c.k_scale; a.vs = (char*)c.v_scale;
-    a.page_bytes = c.page_stride * (c.kind == SS_KV_SAME ? 2 : 1);
-    a.sc_stride = c.scale_stride;
+    a.page_bytes = (unsigned)(c.page_stride * (c.kind == SS_KV_SAME ? 2 : 1));
+    a.sc_stride = (unsigned)c.scale_stride;
     a.table = b.page_table; a.q_start = b.q_start; a.kv_len = b.kv_len; a.table_stride = b.table_stride;
     a.n_pages = c.n_pages; a.page_shift = __builtin_ctz((unsigned)c.page_size); a.H = c.n_kv_heads;
     a.max_pages = b.max_pages; a.n_seqs = b.n_seqs; a.n_tokens = b.n_tokens;
@@ -939,7 +974,7 @@ KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads
     const long rows = (long)b.max_new * G, pairs = (long)b.n_seqs * c.n_kv_heads;
     p.tile = rows > 16;
     p.few = !p.tile || (long)std::max(b.min_new, 1) * G <= 16;
-    p.qc = rows <= 64 ? 1 : 2;
+    p.qc = rows <= 64 ? 1 : rows < 1024 || c.head_dim == 128 ? 2 : 4;
     p.few_keys = p.tile_keys = (int)std::min(keys, 1l << 30);
     auto cut = [&](long groups, long want, int least, int* splits, int* len) {   // as many key ranges as fill the card, none shorter than `least`
         const long n = std::max(1l, std::min({(want + groups - 1) / groups, (keys + least - 1) / least, 64l}));
@@ -992,7 +1027,9 @@ void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv
                 kv_attn_tile_kernel<T, K, D, QC><<<(unsigned)((long)b.n_seqs * c.n_kv_heads * t.nq * p.tile_splits), 256, smem, st>>>(a, t);
                 SS_LAUNCH_CHECK();
             };
-            if (p.qc == 1) go(Int<1>()); else go(Int<2>());
+            if (p.qc == 1) go(Int<1>());
+            else if (p.qc == 2 || D == 128) go(Int<2>());
+            else if constexpr (D == 64) go(Int<4>());
             join(0);
         }
     });
