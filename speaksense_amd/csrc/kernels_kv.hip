@@ -673,51 +673,60 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     for (int i = 0; i < QC; i++) st[i].clear();
     ScaleRef sr;
 
-    // staging: a row of codes is D B / 16 pieces of 16 bytes; thread -> rows tid / PR + i (256 / PR)
+    // staging: a row of codes is PR pieces of 16 bytes; thread -> rows tid / PR + p RP.  The rows that a wave's piece p touches lie in one group of 16 keys,
+    // hence on one page: its address is scalar, the lane's offset the same for all pieces and tiles.
     constexpr int PR = D * B / 16, RP = 256 / PR, NP = 64 / RP;
+    const int group = wave * (64 / PR) / 16;               // of piece 0
+    const unsigned lane_off = (tid / PR & 15) * (D * B) + (tid % PR) * 16;
     u32x4 gk[NP], gv[NP];
-    float gks = 0.0f, gvs = 0.0f;      // threads 0..63: the scales of the tile's rows
-    int id[NP], sid = -1, hid = -1;    // page numbers for the next fetch: of this thread's rows, of its scale row, of 16 keys each (lanes 0..3)
-    unsigned okay = 0;                 // of the fetched tile: bit p = piece p lies on a page, bit 31 = the scales do
+    float gks = 0.0f, gvs = 0.0f;      // first wave: the scales of the tile's rows
+    int hid = -1;                      // lanes 0..3: page numbers for the next fetch, of 16 keys each
+    bool okay = false;                 // of the fetched tile: the scales of this lane's row lie on a page
     int bad = 0;                       // of the fetched tile: bit b = its keys 16 b .. 16 b + 15 lie on no page
     const int mask = (1 << a.page_shift) - 1;
+    const long head_row = (long)h << a.page_shift;
     const int* trow = a.table + (long)s * a.table_stride;
-    auto entry = [&](int key) { return key < sp.len ? trow[key >> a.page_shift] : -1; };          // key < len <= max_pages * page_size
     auto there = [&](int page) { return page >= 0 && page < a.n_pages; };
     auto ids = [&](int i) {
-        const int key0 = lo + i * 64;
-#pragma unroll
-        for (int p = 0; p < NP; p++) id[p] = entry(key0 + tid / PR + p * RP);
-        if (SCALED && wave == 0) sid = entry(key0 + lane);
-        if (lane < 4) hid = entry(key0 + 16 * lane);
+        const int key = lo + i * 64 + 16 * lane;
+        if (lane < 4) hid = key < sp.len ? trow[key >> a.page_shift] : -1;       // key < len <= max_pages * page_size
     };
     auto fetch = [&](int i) {          // tile i; ids(i) has run
         const int key0 = lo + i * 64;
-        okay = 0;
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-            const int key = key0 + tid / PR + p * RP, page = there(id[p]) ? id[p] : 0;
-            if (there(id[p])) okay |= 1u << p;
-            const long off = (long)((unsigned long)(unsigned)page * a.page_bytes) + (((long)h << a.page_shift) + (key & mask)) * (D * B) + (tid % PR) * 16;
-            gk[p] = *(const u32x4*)(a.k + off);
-            gv[p] = *(const u32x4*)(a.v + off);
+            const int b = p * RP / 16 + group, id = __builtin_amdgcn_readlane(hid, b);
+            const long off = (long)((unsigned long)(unsigned)(there(id) ? id : 0) * a.page_bytes) + (head_row + ((key0 + 16 * b) & mask)) * (D * B);
+            gk[p] = *(const u32x4*)(a.k + off + lane_off);
+            gv[p] = *(const u32x4*)(a.v + off + lane_off);
         }
         if (SCALED && wave == 0) {
-            const long at = (long)((unsigned long)(unsigned)(there(sid) ? sid : 0) * a.sc_stride) + ((long)h << a.page_shift) + ((key0 + lane) & mask);
-            if (there(sid)) okay |= 1u << 31;
+            const int id = __shfl(hid, lane >> 4);
+            okay = there(id) && key0 + lane < sp.len;
+            const long at = (long)((unsigned long)(unsigned)(there(id) ? id : 0) * a.sc_stride) + head_row + ((key0 + lane) & mask);
             if constexpr (KIND == K_E4M3) {
                 gks = __uint_as_float((unsigned)(unsigned char)a.ks[at] << 23);
                 gvs = __uint_as_float((unsigned)(unsigned char)a.vs[at] << 23);
             } else { gks = ((const float*)a.ks)[at]; gvs = ((const float*)a.vs)[at]; }
         }
-        bad = (int)__ballot(lane < 4 && key0 + 16 * lane < sp.len && !there(hid));
+        bad = 0;
+#pragma unroll
+        for (int b = 0; b < 4; b++) bad |= key0 + 16 * b < sp.len && !there(__builtin_amdgcn_readlane(hid, b)) ? 1 << b : 0;
     };
-    auto put = [&](char* buf) {
+    auto put = [&](int i, char* buf) { // what fetch(i) brought
+        const int key0 = lo + i * 64;
+        if (key0 + 64 > sp.len || bad) {                   // values of no key: whatever lies there must not meet a probability of 0
+            asm volatile("");
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                const int r = tid / PR + p * RP;
+                if (key0 + r >= sp.len || (bad >> (r >> 4) & 1)) gv[p] = (u32x4){0, 0, 0, 0};
+            }
+        }
 #pragma unroll
         for (int p = 0; p < NP; p++) {
             const int r = tid / PR + p * RP;
             char *kd = buf + r * KP, *vd = buf + 64 * KP + r * VP;
-            if (!(okay >> p & 1)) gv[p] = (u32x4){0, 0, 0, 0};     // whatever lies there must not meet a probability of 0
             if constexpr (!SCALED) {
                 *(u32x4*)(kd + (tid % PR) * 16) = gk[p];
                 *(u32x4*)(vd + (tid % PR) * 16) = gv[p];
@@ -725,21 +734,21 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
                 u32x4 x[2];
                 unsigned o[2];
 #pragma unroll
-                for (int i = 0; i < 4; i++) { codes_to_f16<KIND>(gk[p][i], o); x[i >> 1][2 * (i & 1)] = o[0]; x[i >> 1][2 * (i & 1) + 1] = o[1]; }
+                for (int w = 0; w < 4; w++) { codes_to_f16<KIND>(gk[p][w], o); x[w >> 1][2 * (w & 1)] = o[0]; x[w >> 1][2 * (w & 1) + 1] = o[1]; }
                 *(u32x4*)(kd + (tid % PR) * 32) = x[0];
                 *(u32x4*)(kd + (tid % PR) * 32 + 16) = x[1];
 #pragma unroll
-                for (int i = 0; i < 4; i++) { codes_to_f16<KIND>(gv[p][i], o); x[i >> 1][2 * (i & 1)] = o[0]; x[i >> 1][2 * (i & 1) + 1] = o[1]; }
+                for (int w = 0; w < 4; w++) { codes_to_f16<KIND>(gv[p][w], o); x[w >> 1][2 * (w & 1)] = o[0]; x[w >> 1][2 * (w & 1) + 1] = o[1]; }
                 *(u32x4*)(vd + (tid % PR) * 32) = x[0];
                 *(u32x4*)(vd + (tid % PR) * 32 + 16) = x[1];
             }
         }
         if (SCALED && wave == 0) {     // the first wave keeps sref and hands out what follows from it
             float* sc = (float*)(buf + 64 * (KP + VP));
-            const float v = okay >> 31 ? gvs : 0.0f;
+            const float v = okay ? gvs : 0.0f;
             float by = 1.0f;
             sr.moves(v, &by);
-            sc[lane] = okay >> 31 ? gks : 0.0f;
+            sc[lane] = okay ? gks : 0.0f;
             sc[64 + lane] = v * sr.inv();
             if (lane == 0) { sc[128] = sr.ref; sc[129] = by; }
         }
@@ -840,7 +849,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
         fetch(0);
         hole = bad;
         if (n > 1) ids(1);
-        put(smem);
+        put(0, smem);
         if (n > 1) fetch(1);
         if (n > 2) ids(2);
         __syncthreads();
@@ -849,7 +858,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
             if (key0 < wend) compute(key0 + 64 > full || hole, smem + (i & 1) * kBuf, key0);
             if (++i >= n) break;
             hole = bad;
-            put(smem + (i & 1) * kBuf);                    // last read before the barrier that ended tile i - 2
+            put(i, smem + (i & 1) * kBuf);                 // last read before the barrier that ended tile i - 2
             if (i + 1 < n) fetch(i + 1);
             if (i + 2 < n) ids(i + 2);
             __syncthreads();
