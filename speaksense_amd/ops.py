@@ -71,8 +71,11 @@ def _on(t, device, name):
     _need(device is None or t.device == device, f"{name} is on {t.device}, expected {device}")
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):      # 0.1 us; the public way builds a Stream object for 2
+    _stream = torch._C._cuda_getCurrentRawStream
+else:
+    def _stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 class KvCache:
@@ -103,7 +106,7 @@ class KvCache:
                 _on(t, k.device, name)
                 _need(t.dtype == scales and t.shape == k.shape[:3], f"{name} must be {scales} [n_pages, n_kv_heads, page_size]")
                 _need(t.stride()[1:] == (page, 1) and t.stride(0) == k_scale.stride(0), "each page's scales must be contiguous, with one stride between pages")
-        self.k, self.v, self.k_scale, self.v_scale, self.dtype, self.device = k, v, k_scale, v_scale, dtype, k.device
+        self.k, self.v, self.k_scale, self.v_scale, self.dtype, self.device, self.index = k, v, k_scale, v_scale, dtype, k.device, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, heads, page, dim
         # a cache of one page may be a view whose stride says nothing
         page_stride = k.stride(0) if n > 1 else max(k.stride(0), heads * page * dim)
@@ -140,31 +143,37 @@ class KvBatch:
         _need(kv_len.numel() == n and q_start.numel() == n + 1, f"{n} rows of page_table, {kv_len.numel()} lengths, {q_start.numel()} starts")
         _need((pages <= 1 or page_table.stride(1) == 1) and (n == 0 or (kv_len.is_contiguous() and q_start.is_contiguous())), "rows of page_table, q_start and kv_len must be contiguous")
         _need(all(isinstance(x, int) and 0 <= x < 1 << 31 for x in (n_tokens, max_new, min_new, max_len)), "n_tokens, max_new, min_new and max_len must be host integers in [0, 2^31)")
-        self.page_table, self.q_start, self.kv_len, self.device = page_table, q_start, kv_len, page_table.device
+        self.page_table, self.q_start, self.kv_len, self.device, self.index = page_table, q_start, kv_len, page_table.device, page_table.get_device()
         self.n_seqs, self.n_tokens, self.max_new = n, n_tokens, max_new
         stride = page_table.stride(0) if n > 1 else pages
         self._c = _Batch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride, n, pages, n_tokens, max_new, min_new, max_len)
 
 
 def _rows(t, name, cache, batch, heads):
+    """The C view of token rows [n_tokens, heads, head_dim]; `heads` None: any number."""
+    if isinstance(t, torch.Tensor) and t.dtype is cache.dtype and t.get_device() == cache.index:
+        shape = t.shape
+        if len(shape) == 3 and shape[0] == batch.n_tokens and shape[2] == cache.head_dim and (heads is None or shape[1] == heads):
+            row, head, element = t.stride()
+            if element == 1:       # a stride over one row or one head says nothing
+                return _Rows(t.data_ptr(), row if shape[0] > 1 else cache.head_dim * shape[1], head if shape[1] > 1 else cache.head_dim)
     _on(t, cache.device, name)
     _need(t.dtype == cache.dtype, f"{name} must be {cache.dtype}, got {t.dtype}")
     _need(t.dim() == 3 and t.shape[0] == batch.n_tokens and t.shape[2] == cache.head_dim and (heads is None or t.shape[1] == heads),
           f"{name} must be [{batch.n_tokens}, {'n_heads' if heads is None else heads}, {cache.head_dim}], got {list(t.shape)}")
-    _need(t.stride(2) == 1, f"the elements of a head of {name} must be contiguous")
-    return _Rows(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else cache.head_dim * t.shape[1], t.stride(1) if t.shape[1] > 1 else cache.head_dim)
+    raise ValueError(f"the elements of a head of {name} must be contiguous")
 
 
 def _same_device(cache, batch):
     _need(isinstance(cache, KvCache) and isinstance(batch, KvBatch), "expected a KvCache and a KvBatch")
-    _need(batch.device == cache.device, f"the batch is on {batch.device}, the cache on {cache.device}")
+    _need(batch.index == cache.index, "the batch and the cache are on different devices")
 
 
 def kv_append(cache: KvCache, batch: KvBatch, k, v) -> None:
     """Write the new tokens' keys and values [n_tokens, n_kv_heads, head_dim] into their pages, in the cache's form (ss_kv_append)."""
     _same_device(cache, batch)
     kr, vr = _rows(k, "k", cache, batch, cache.n_kv_heads), _rows(v, "v", cache, batch, cache.n_kv_heads)
-    binding._check(_lib().ss_kv_append(cache._c, batch._c, kr, vr, cache.device.index, _stream(cache.device)))
+    binding._check(_lib().ss_kv_append(cache._c, batch._c, kr, vr, cache.index, _stream(cache.index)))
 
 
 def kv_read(cache: KvCache, batch: KvBatch, out=None):
@@ -175,7 +184,7 @@ def kv_read(cache: KvCache, batch: KvBatch, out=None):
         out = tuple(torch.empty((batch.n_tokens, cache.n_kv_heads, cache.head_dim), dtype=cache.dtype, device=cache.device) for _ in "kv")
     k, v = out
     kr, vr = _rows(k, "out[0]", cache, batch, cache.n_kv_heads), _rows(v, "out[1]", cache, batch, cache.n_kv_heads)
-    binding._check(_lib().ss_kv_read(cache._c, batch._c, kr, vr, cache.device.index, _stream(cache.device)))
+    binding._check(_lib().ss_kv_read(cache._c, batch._c, kr, vr, cache.index, _stream(cache.index)))
     return k, v
 
 
@@ -195,7 +204,7 @@ def kv_attention(cache: KvCache, batch: KvBatch, q, *, scale=None, causal=True, 
         binding._check(int(need))
     work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     binding._check(L.ss_kv_attention(cache._c, batch._c, qr, heads, cache.head_dim ** -0.5 if scale is None else float(scale), 1 if causal else 0, orow,
-                                     lse.data_ptr() if return_lse else None, work.data_ptr() if need else None, need, cache.device.index, _stream(cache.device)))
+                                     lse.data_ptr() if return_lse else None, work.data_ptr() if need else None, need, cache.index, _stream(cache.index)))
     return (out, lse) if return_lse else out
 
 
@@ -210,7 +219,7 @@ def sample_rows(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
     """One id per row of logits [n_rows, n_vocab] (float32, float16 or bfloat16) from uniform numbers u [n_rows] (float64): temperature, top-k, top-p and
     min-p per row (ss_sample_rows).  Each setting is a tensor [n_rows] (float32; top_k int32) on the device, or None for "off"."""
     _on(logits, None, "logits")
-    dev = logits.device
+    dev, index = logits.device, logits.get_device()
     _need(logits.dtype in _DTYPES, f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
     _need(logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1), "logits must be [n_rows, n_vocab] with contiguous rows")
     n, v = logits.shape
@@ -220,12 +229,14 @@ def sample_rows(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
         if t is None and name != "u":
             ptr.append(None)
             continue
-        _on(t, dev, name)
-        _need(t.dtype == dt and t.shape == (n,) and t.is_contiguous(), f"{name} must be {dt} [{n}], contiguous")
+        if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dt and t.shape == (n,) and t.is_contiguous()):
+            _on(t, dev, name)
+            raise ValueError(f"{name} must be {dt} [{n}], contiguous")
         ptr.append(t.data_ptr())
-    whole = torch.empty((2, n), dtype=torch.int32, device=dev)
-    real = torch.empty((2, n), dtype=torch.float32, device=dev)
-    r = Sampled(whole[0], real[0], real[1], whole[1])
-    a = _Sample(*ptr, r.id.data_ptr(), r.p.data_ptr(), r.logprob.data_ptr(), r.n_kept.data_ptr(), logits.stride(0) if n > 1 else v, n, v, _DTYPES[logits.dtype], 0)
-    binding._check(_lib().ss_sample_rows(a, dev.index, _stream(dev)))
-    return r
+    whole, real = torch.empty((2, n), dtype=torch.int32, device=dev), torch.empty((2, n), dtype=torch.float32, device=dev)
+    ids, kept = whole.unbind()
+    p, logprob = real.unbind()
+    w, f = whole.data_ptr(), real.data_ptr()
+    a = _Sample(*ptr, w, f, f + 4 * n, w + 4 * n, logits.stride(0) if n > 1 else v, n, v, _DTYPES[logits.dtype], 0)
+    binding._check(_lib().ss_sample_rows(a, index, _stream(index)))
+    return Sampled(ids, p, logprob, kept)
