@@ -3,7 +3,7 @@
 // With max = the row's largest logit and c = log2(e) / t, id i weighs 2^((x_i - max) c), held as an integer W_i = round(w_i 2^S), S = 62 - ceil(log2 n_vocab)
 // (at most 51): every sum of a row fits 62 bits and is exact, so neither the order of the atomics nor the split over waves can change a result, and a running
 // sum is compared with u times the total exactly.  The exponential is evaluated in double: 2^y = 2^(k/256) 2^r, k = round(256 y), |r| <= 1/512, the first
-// factor from a table, the second from its series up to r^4 (the next term is 2e-17).
+// factor from a table, the second from its series up to r^3 (the next term is below 1.4e-13 of it).
 //
 // top-k and top-p are both "keep an id while the measure of the better ones stays below a target", the measure being 1 or W: a histogram over
 // 2048 equal steps of the logit finds the step in which the target is crossed, the ids of that step are gathered into LDS and ranked there exactly by
@@ -19,12 +19,10 @@ namespace ss {
 namespace {
 
 typedef unsigned long long u64;
-constexpr int kWaves = 16, kThreads = 64 * kWaves, kBins = 2048, kList = 1024;
+constexpr int kBins = 2048, kList = 1024;
 constexpr float kInf = __builtin_huge_valf();
-constexpr unsigned kKeyNegInf = 0x007fffffu;     // order_key(-inf): every masked id has this key or a lower one
-
 __device__ __forceinline__ unsigned order_key(float x) {   // larger number <=> larger key
-    const unsigned u = __float_as_uint(x);
+    const unsigned u = __float_as_uint(x + 0.0f);           // -0 -> +0: equal numbers get equal keys
     return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 
@@ -38,15 +36,20 @@ template <typename T> struct Row {
     int n, groups;
     bool inf_row;                  // the largest logit is +inf: only those ids count, all alike
     __device__ __forceinline__ float clean(T v) const {
-        float x = (float)v + 0.0f;                       // -0 -> +0: equal numbers get equal keys
-        x = x != x ? -kInf : x;
+        const float x = fmaxf((float)v, -kInf);          // NaN counts as masked
         return inf_row ? (x == kInf ? 0.0f : -kInf) : x;
     }
-    // this lane's VEC consecutive ids of group g: x[], first id returned; ids behind the row are masked
-    __device__ __forceinline__ int load(int g, int lane, float* x) const {
+    // this lane's VEC consecutive ids of group g, as they lie in memory; a lane that the row's end cuts reads nothing here
+    __device__ __forceinline__ V fetch(int g, int lane) const {
+        const int i0 = g * GROUP + lane * VEC;
+        V v{};
+        if (i0 + VEC <= n) v = *(const V*)(p + i0);
+        return v;
+    }
+    // their values x[]; ids behind the row are masked; returns the first id
+    __device__ __forceinline__ int values(int g, int lane, V v, float* x) const {
         const int i0 = g * GROUP + lane * VEC;
         if (i0 + VEC <= n) {
-            const V v = *(const V*)(p + i0);
 #pragma unroll
             for (int e = 0; e < VEC; e++) x[e] = clean(v[e]);
         } else {
@@ -55,33 +58,44 @@ template <typename T> struct Row {
         }
         return i0;
     }
+    __device__ __forceinline__ int load(int g, int lane, float* x) const { return values(g, lane, fetch(g, lane), x); }
 };
 
-struct Weight {                    // w(x) in double and as an integer
-    const double* table;           // LDS: 2^(j/256)
-    double max, c, one;            // one = 2^S
-    int S;
-    __device__ __forceinline__ double scaled(float x) const {            // w 2^S
-        const double y = fmax(((double)x - max) * c, -1000.0);
+struct Weight {                    // w(x) 2^S in double and as an integer
+    const double* table;           // LDS: 2^(j/256 + S)
+    double top, c, least;          // y = (x - top) c; below `least` w 2^S is less than 2^-16 and counts as that, which rounds to 0
+    __device__ __forceinline__ double scaled(float x) const {
+        const double y = fmax(((double)x - top) * c, least);
         constexpr double magic = 6755399441055744.0 / 256.0;             // 1.5 2^52 / 256: adding it rounds y to a multiple of 1/256
         const double z = y + magic;
         const int k = (int)(unsigned)__double_as_longlong(z);            // low word of the mantissa: 256 y, rounded, two's complement
         const double r = y - (z - magic);
-        constexpr double L1 = 0.693147180559945309417, L2 = 0.240226506959100712333, L3 = 0.0555041086648215799532, L4 = 0.00961812910762847716198;
-        const double q = r * (L1 + r * (L2 + r * (L3 + r * L4)));
+        constexpr double L1 = 0.693147180559945309417, L2 = 0.240226506959100712333, L3 = 0.0555041086648215799532;
+        const double q = r * fma(r, fma(r, L3, L2), L1);
         const double t = table[k & 255];
-        return ldexp(t + t * q, (k >> 8) + S);
+        const double s = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));   // the exponent: -16 <= k / 256 + S <= 51
+        return fma(s, q, s);
     }
     static __device__ __forceinline__ u64 integer(double s) {            // round(s), 0 <= s <= 2^51
         return (u64)__double_as_longlong(s + 4503599627370496.0) & 0x000fffffffffffffull;
     }
 };
 
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int o) { return (u64)__shfl_xor((unsigned long long)v, o); }
+template <int CTRL> __device__ __forceinline__ u64 add_dpp64(u64 v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, 0xf, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, 0xf, 0xf, false);
+    return v + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 lane64(u64 v, int l) {
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), l) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, l);
+}
+// on the VALU (a shuffle is a round trip through LDS); the same in every lane
 __device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += shfl_xor64(v, o);
-    return v;
+    v = add_dpp64<kDppRor8>(v);
+    v = add_dpp64<kDppRor4>(v);
+    v = add_dpp64<kDppXor2>(v);
+    v = add_dpp64<kDppXor1>(v);
+    return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
 }
 __device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {            // inclusive
 #pragma unroll
@@ -92,41 +106,58 @@ __device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {            // incl
     return v;
 }
 
-struct Shared {
+template <int THREADS> struct Shared {
     double table[256];
     u64 hist[kBins];
-    Entry list[kList];
-    u64 wave64[kWaves + 1];
-    float wave_f[3][kWaves];
-    int wave_i[kWaves];
+    Entry list[kList];             // the ids of the step in which a target is crossed
+    Entry kept[kList];             // the ids above it, and of it those that stay: everything that is kept, if it fits
+    u64 wave64[THREADS / 64 + 1];
+    float wave_f[2][THREADS / 64];
+    int wave_i[THREADS / 64];
     u64 found_base;
     unsigned found_key, key_lo, key_hi;
-    int found, found_id, n_list;
+    int found, found_id, n_list, n_kept;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_args a, int S) {
-    __shared__ Shared sh;
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_args a, int S) {
+    constexpr int WAVES = THREADS / 64, BPT = kBins / THREADS;
+    __shared__ Shared<THREADS> sh;
     extern __shared__ __attribute__((aligned(16))) char dyn[];
     u64* mass = (u64*)dyn;                                               // [groups] measure of each group's kept ids
     typedef Row<T> R;
-    constexpr int VEC = R::VEC;
+    constexpr int VEC = R::VEC, AHEAD = 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
     R r{(const T*)a.logits + (long)row * a.row_stride, a.n_vocab, (a.n_vocab + R::GROUP - 1) / R::GROUP, false};
-    for (int i = tid; i < 256; i += kThreads) sh.table[i] = exp2(i * (1.0 / 256.0));
+
+    // f(group, first id of the lane, its VEC logits) over the wave's groups, the loads of the next AHEAD groups in flight.  f appears once in a rolled
+    // loop: a workgroup runs through its code only a few times, and instruction fetches cost more than the moves between the buffers.
+    auto over_row = [&](auto f) {
+        typename R::V v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) v[i] = r.fetch(wave + i * WAVES, lane);
+#pragma unroll 1
+        for (int g = wave; g < r.groups; g += WAVES) {
+            float x[VEC];
+            const int i0 = r.values(g, lane, v[0], x);
+#pragma unroll
+            for (int i = 0; i + 1 < AHEAD; i++) v[i] = v[i + 1];
+            v[AHEAD - 1] = r.fetch(g + AHEAD * WAVES, lane);
+            f(g, i0, x);
+        }
+    };
 
     // the largest logit (lowest id), the smallest unmasked one
     float top = -kInf, low = kInf;
     int best = 0x7fffffff;
-    for (int g = wave; g < r.groups; g += kWaves) {
-        float x[VEC];
-        const int i0 = r.load(g, lane, x);
+    over_row([&](int, int i0, const float* x) {
 #pragma unroll
         for (int e = 0; e < VEC; e++) {
             if (x[e] > top) { top = x[e]; best = i0 + e; }
-            if (x[e] > -kInf) low = fminf(low, x[e]);
+            low = fminf(low, x[e] > -kInf ? x[e] : kInf);
         }
-    }
+    });
+    for (int i = tid; i < 256; i += THREADS) sh.table[i] = exp2(i * (1.0 / 256.0) + S);
     {
         const float wt = wave_max(top);
         int wb = top == wt ? best : 0x7fffffff;
@@ -137,7 +168,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     }
     __syncthreads();
     top = -kInf; best = 0x7fffffff; low = kInf;
-    for (int w = 0; w < kWaves; w++) {
+    for (int w = 0; w < WAVES; w++) {
         const float t = sh.wave_f[0][w];
         const int b = sh.wave_i[w];
         if (t > top) { top = t; best = b; } else if (t == top) best = min(best, b);
@@ -158,37 +189,43 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     const bool greedy = !(t_row > 0.0f);
     // an infinite or vanishing t must not meet a difference of 0 or infinity
     const double c = fmax(fmin(1.44269504088896340736 / (greedy ? 1.0 : (double)t_row), 1e300), 1e-300);
-    const Weight wt{sh.table, (double)top, c, ldexp(1.0, S), S};
+    const double one = ldexp(1.0, S);
+    const Weight wt{sh.table, (double)top, c, -(double)(S + 16)};
     const int k_row = a.top_k ? a.top_k[row] : 0;
     const float p_row = a.top_p ? a.top_p[row] : 1.0f;
     const bool by_k = !greedy && k_row > 0 && k_row < a.n_vocab, by_p = !greedy && p_row < 1.0f;
     float m_row = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
     if (a.min_p && !(a.min_p[row] == a.min_p[row])) m_row = 0.0f;
     const bool by_m = !greedy && m_row > 0.0f;
-    const double m_scaled = (double)m_row * wt.one;
+    const double m_scaled = (double)m_row * one;
 
-    // the sum of all weights, for logprob, where the exact total of the kept ones is not that
+    // the sum of all weights, for logprob: of float32 exponentials where some pass goes over the whole row and needs no exact ones, else exact
+    float part = 0.0f;
     double whole = 0.0;
-    auto block_sum = [&](float v) {
-        const double s = (double)wave_sum(v);
+    const float cf = (float)c;
+    const bool plain = c > 1e-30 && c < 1e30;                             // float32 takes it
+    auto add_parts = [&](const float* x) {
+        if (plain)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) part += __builtin_amdgcn_exp2f((x[e] - top) * cf);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; e++) part += __builtin_amdgcn_exp2f((float)((double)(x[e] - top) * c));
+    };
+    auto sum_parts = [&]() {
+        const double s = (double)wave_sum(part);
         __syncthreads();
         if (lane == 0) sh.wave64[wave] = (u64)__double_as_longlong(s);
         __syncthreads();
-        double z = 0.0;
-        for (int w = 0; w < kWaves; w++) z += __longlong_as_double((long long)sh.wave64[w]);
-        return z;
+        whole = 0.0;
+        for (int w = 0; w < WAVES; w++) whole += __longlong_as_double((long long)sh.wave64[w]);
+        __syncthreads();
     };
-    if (a.logprob && (greedy || by_k || by_p || by_m)) {
-        float s = 0.0f;
-        for (int g = wave; g < r.groups; g += kWaves) {
-            float x[VEC];
-            r.load(g, lane, x);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) s += __builtin_amdgcn_exp2f((float)((double)(x[e] - top) * c));
-        }
-        whole = block_sum(s);
-    }
     if (greedy) {
+        if (a.logprob) {
+            over_row([&](int, int, const float* x) { add_parts(x); });
+            sum_parts();
+        }
         if (tid == 0) {
             a.id[row] = best;
             if (a.p) a.p[row] = 1.0f;
@@ -199,88 +236,122 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     }
     __syncthreads();                                                      // the table
 
-    unsigned thr = kKeyNegInf;                                            // kept: key > thr, or key == thr and id <= thr_id
+    float thr = -kInf;                                                    // kept: x > thr, or x == thr and id <= thr_id
     int thr_id = -1;
-    auto alive = [&](unsigned key, int id) { return key > thr || (key == thr && id <= thr_id); };
+    auto alive = [&](float x, int id) { return x > thr || (x == thr && id <= thr_id); };
     const float steps = low < top ? (float)(kBins - 1) / (top - low) : 0.0f;
     auto bin_of = [&](float x) { return min((int)((top - x) * steps), kBins - 1); };
+    auto value_of = [&](unsigned key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); };
 
-    // finds the crossing of `target` in hist (bins in order from the best): bin in sh.found, measure before it in sh.found_base; the total is returned
-    auto total_of_hist = [&]() {
-        u64 v = sh.hist[2 * tid] + sh.hist[2 * tid + 1];
+    auto block_sum64 = [&](u64 v) {
         v = wave_sum64(v);
+        __syncthreads();
         if (lane == 0) sh.wave64[wave] = v;
         __syncthreads();
         u64 t = 0;
-        for (int w = 0; w < kWaves; w++) t += sh.wave64[w];
+        for (int w = 0; w < WAVES; w++) t += sh.wave64[w];
         __syncthreads();
         return t;
     };
-    auto cross = [&](u64 base, u64 target) {
-        const u64 h0 = sh.hist[2 * tid], h1 = sh.hist[2 * tid + 1];
-        const u64 inc = wave_scan64(h0 + h1, lane);
-        if (lane == 63) sh.wave64[wave] = inc;
-        __syncthreads();
-        u64 before = base + inc - (h0 + h1);
-        for (int w = 0; w < wave; w++) before += sh.wave64[w];
-        if (before < target && target <= before + h0) { sh.found = 2 * tid; sh.found_base = before; }
-        before += h0;
-        if (before < target && target <= before + h1) { sh.found = 2 * tid + 1; sh.found_base = before; }
-        __syncthreads();
-    };
-    // narrows (thr, thr_id) to the ids whose better ones measure less than the target
+    bool listed = false;               // sh.kept holds every kept id
+    // narrows (thr, thr_id) to the ids whose better ones measure less than the target.  The ids come from the row, or from sh.kept where that has them all.
     auto select = [&](auto by_mass, u64 count) {
         constexpr bool MASS = decltype(by_mass)::value;
         auto measure = [&](float x) -> u64 { return MASS ? Weight::integer(wt.scaled(x)) : 1; };
-        auto fill = [&](auto bin) {                                       // bin(x, key): bin or -1
+        const bool from_list = listed;
+        const int n_from = listed ? sh.n_kept : 0;
+        auto each = [&](auto f) {                                         // f(logit, id) of every id still kept
+            if (from_list) {
+                for (int i = tid; i < n_from; i += THREADS) f(value_of(sh.kept[i].key), sh.kept[i].id);
+            } else {
+                over_row([&](int, int i0, const float* x) {
+#pragma unroll
+                    for (int e = 0; e < VEC; e++)
+                        if (alive(x[e], i0 + e)) f(x[e], i0 + e);
+                });
+            }
+        };
+        // counts need 32 bits: half the LDS traffic
+        auto add = [&](int bin, float x) {
+            if constexpr (MASS) atomicAdd(&sh.hist[bin], measure(x));
+            else atomicAdd((unsigned*)sh.hist + bin, 1u);
+        };
+        auto bin_at = [&](int i) -> u64 { return MASS ? sh.hist[i] : (u64)((const unsigned*)sh.hist)[i]; };
+        auto my_bins = [&]() {
+            u64 s = 0;
+#pragma unroll
+            for (int i = 0; i < BPT; i++) s += bin_at(BPT * tid + i);
+            return s;
+        };
+        // finds the crossing of `target` in hist (bins in order from the best): bin in sh.found, measure before it in sh.found_base
+        auto cross = [&](u64 base, u64 target) {
+            const u64 mine = my_bins(), inc = wave_scan64(mine, lane);
+            if (lane == 63) sh.wave64[wave] = inc;
             __syncthreads();
-            sh.hist[2 * tid] = 0; sh.hist[2 * tid + 1] = 0;
+            u64 before = base + inc - mine;
+            for (int w = 0; w < wave; w++) before += sh.wave64[w];
+#pragma unroll
+            for (int i = 0; i < BPT; i++) {
+                const u64 h = bin_at(BPT * tid + i);
+                if (before < target && target <= before + h) { sh.found = BPT * tid + i; sh.found_base = before; }
+                before += h;
+            }
+            __syncthreads();
+        };
+        auto clear = [&]() {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < BPT; i++) sh.hist[BPT * tid + i] = 0;
             if (tid == 0) { sh.n_list = 0; sh.key_lo = 0xffffffffu; sh.key_hi = 0; sh.found = -1; }
             __syncthreads();
-            for (int g = wave; g < r.groups; g += kWaves) {
-                float x[VEC];
-                const int i0 = r.load(g, lane, x);
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const unsigned key = order_key(x[e]);
-                    if (!alive(key, i0 + e)) continue;
-                    const int b = bin(x[e], key);
-                    if (b >= 0) atomicAdd(&sh.hist[b], measure(x[e]));
-                }
-            }
-            __syncthreads();
         };
-        auto gather = [&](auto in) {
-            for (int g = wave; g < r.groups; g += kWaves) {
-                float x[VEC];
-                const int i0 = r.load(g, lane, x);
-#pragma unroll
-                for (int e = 0; e < VEC; e++) {
-                    const unsigned key = order_key(x[e]);
-                    if (!alive(key, i0 + e) || !in(x[e], key)) continue;
-                    const int at = atomicAdd(&sh.n_list, 1);
-                    if (at < kList) sh.list[at] = Entry{key, i0 + e, measure(x[e])};
-                    atomicMin(&sh.key_lo, key);
-                    atomicMax(&sh.key_hi, key);
-                }
-            }
-            __syncthreads();
+        auto take = [&](float x, int id) {                                // into the list of candidates
+            const unsigned key = order_key(x);
+            const int at = atomicAdd(&sh.n_list, 1);
+            if (at < kList) sh.list[at] = Entry{key, id, measure(x)};
+            atomicMin(&sh.key_lo, key);
+            atomicMax(&sh.key_hi, key);
         };
-        fill([&](float x, unsigned) { return bin_of(x); });
-        const u64 total = total_of_hist();
+        clear();
+        if (!MASS && a.logprob) {      // the pass that counts also sums up what logprob needs
+            over_row([&](int, int i0, const float* x) {
+                add_parts(x);
+#pragma unroll
+                for (int e = 0; e < VEC; e++)
+                    if (x[e] > -kInf) add(bin_of(x[e]), x[e]);
+            });
+        } else each([&](float x, int) { add(bin_of(x), x); });
+        __syncthreads();
+        if (!MASS && a.logprob) sum_parts();
+        const u64 total = block_sum64(my_bins());
+        if (MASS && !by_k) whole = (double)total / one;
         u64 target = count;
         if constexpr (MASS) target = max((u64)1, (u64)ceil((double)fmaxf(p_row, 0.0f) * (double)total));
         if (target >= total) return;                                      // all of them
         cross(0, target);
         int b = sh.found;
         u64 base = sh.found_base;
-        gather([&](float x, unsigned) { return bin_of(x) == b; });
+        if (from_list) each([&](float x, int id) { if (bin_of(x) == b) take(x, id); });
+        else {
+            if (tid == 0) sh.n_kept = 0;
+            __syncthreads();
+            each([&](float x, int id) {
+                const int y = bin_of(x);
+                if (y == b) take(x, id);
+                else if (y < b) {
+                    const int at = atomicAdd(&sh.n_kept, 1);
+                    if (at < kList) sh.kept[at] = Entry{order_key(x), id, 0};
+                }
+            });
+        }
+        __syncthreads();
+        const bool first = sh.n_list <= kList;                            // the candidates are all of one histogram step
         for (;;) {
             const int n = sh.n_list;
             const unsigned lo = sh.key_lo, hi = sh.key_hi;
             __syncthreads();
             if (n <= kList) {
-                for (int i = tid; i < n; i += kThreads) {
+                for (int i = tid; i < n; i += THREADS) {
                     const Entry me = sh.list[i];
                     u64 before = base;
                     for (int j = 0; j < n; j++)
@@ -288,48 +359,64 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
                     if (before < target && target <= before + me.w) { sh.found_key = me.key; sh.found_id = me.id; }
                 }
                 __syncthreads();
-                thr = sh.found_key; thr_id = sh.found_id;
+                thr = value_of(sh.found_key); thr_id = sh.found_id;
+                if (!from_list && first) {
+                    for (int i = tid; i < n; i += THREADS)
+                        if (alive(value_of(sh.list[i].key), sh.list[i].id)) {
+                            const int at = atomicAdd(&sh.n_kept, 1);
+                            if (at < kList) sh.kept[at] = sh.list[i];
+                        }
+                    __syncthreads();
+                    listed = sh.n_kept <= kList;
+                }
                 return;
             }
             if (lo == hi) {                                               // equal logits: the first `need` of them by id
-                const float x0 = __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
-                const u64 m = measure(x0), need = (target - base + m - 1) / m;
-                auto ties = [&](int g) {                                  // this lane's ties of group g
-                    float x[VEC];
-                    const int i0 = r.load(g, lane, x);
+                const float tie = value_of(lo);
+                const u64 m = measure(tie), need = (target - base + m - 1) / m;
+                auto ties = [&](int i0, const float* x) {                 // this lane's ties of a group
                     int n = 0;
 #pragma unroll
-                    for (int e = 0; e < VEC; e++) n += order_key(x[e]) == lo && alive(lo, i0 + e);
+                    for (int e = 0; e < VEC; e++) n += x[e] == tie && alive(tie, i0 + e);
                     return n;
                 };
-                for (int g = wave; g < r.groups; g += kWaves) {
-                    const u64 n = wave_sum64((u64)ties(g));
+                over_row([&](int g, int i0, const float* x) {
+                    const u64 n = wave_sum64((u64)ties(i0, x));
                     if (lane == 0) mass[g] = n;
-                }
+                });
                 __syncthreads();
                 if (wave == 0) {
                     u64 run = 0;
                     int at = 0;
                     for (; at < r.groups - 1 && run + mass[at] < need; at++) run += mass[at];
-                    const u64 mine = (u64)ties(at), inc = run + wave_scan64(mine, lane);
+                    float x[VEC];
+                    const int i0 = r.load(at, lane, x);
+                    const u64 mine = (u64)ties(i0, x), inc = run + wave_scan64(mine, lane);
                     if (inc - mine < need && need <= inc) {
-                        float x[VEC];
-                        const int i0 = r.load(at, lane, x);
                         u64 n = inc - mine;
 #pragma unroll
                         for (int e = 0; e < VEC; e++)
-                            if (order_key(x[e]) == lo && alive(lo, i0 + e) && ++n == need) sh.found_id = i0 + e;
+                            if (x[e] == tie && alive(tie, i0 + e) && ++n == need) sh.found_id = i0 + e;
                     }
                 }
                 __syncthreads();
-                thr = lo; thr_id = sh.found_id;
+                thr = tie; thr_id = sh.found_id;
                 return;
             }
             const int shift = max(0, 32 - __clz(hi - lo) - 11);
-            fill([&](float, unsigned key) { return key < lo || key > hi ? -1 : (int)((hi - key) >> shift); });
+            clear();
+            each([&](float x, int) {
+                const unsigned key = order_key(x);
+                if (key >= lo && key <= hi) add((int)((hi - key) >> shift), x);
+            });
+            __syncthreads();
             cross(base, target);
             b = sh.found; base = sh.found_base;
-            gather([&](float, unsigned key) { return key >= lo && key <= hi && (int)((hi - key) >> shift) == b; });
+            each([&](float x, int id) {
+                const unsigned key = order_key(x);
+                if (key >= lo && key <= hi && (int)((hi - key) >> shift) == b) take(x, id);
+            });
+            __syncthreads();
         }
     };
     if (by_k) select(std::integral_constant<bool, false>(), (u64)k_row);
@@ -337,32 +424,40 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
 
     // the kept ids' weights, group by group
     auto kept = [&](float x, int id, u64* w) {
-        if (!alive(order_key(x), id)) return false;
+        if (!alive(x, id)) return false;
         const double s = wt.scaled(x);
         *w = Weight::integer(s);
-        return !by_m || s >= m_scaled;
+        return !by_m || s >= m_scaled || x == top;
     };
     __syncthreads();
     u64 total = 0;
     int n_kept = 0;
-    for (int g = wave; g < r.groups; g += kWaves) {
-        float x[VEC];
-        const int i0 = r.load(g, lane, x);
-        u64 s = 0;
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
+    if (listed) {
+        for (int g = tid; g < r.groups; g += THREADS) mass[g] = 0;
+        __syncthreads();
+        for (int i = tid; i < sh.n_kept; i += THREADS) {
+            const Entry e = sh.kept[i];
             u64 w;
-            if (kept(x[e], i0 + e, &w)) { s += w; n_kept++; }
+            if (kept(value_of(e.key), e.id, &w)) { total += w; n_kept++; atomicAdd(&mass[e.id / R::GROUP], w); }
         }
-        s = wave_sum64(s);
-        if (lane == 0) mass[g] = s;
-        total += s;
+    } else {
+        const bool add_whole = a.logprob && by_m && !by_k && !by_p;
+        over_row([&](int g, int i0, const float* x) {
+            u64 s = 0;
+            if (add_whole) add_parts(x);
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                u64 w;
+                if (kept(x[e], i0 + e, &w)) { s += w; n_kept++; }
+            }
+            total += s;
+            s = wave_sum64(s);
+            if (lane == 0) mass[g] = s;
+        });
+        if (add_whole) sum_parts();
     }
-    n_kept = (int)wave_sum((float)n_kept);                                // < 2^24: exact
-    if (lane == 0) { sh.wave64[wave] = total; sh.wave_i[wave] = n_kept; }
-    __syncthreads();
-    total = 0; n_kept = 0;
-    for (int w = 0; w < kWaves; w++) { total += sh.wave64[w]; n_kept += sh.wave_i[w]; }
+    total = block_sum64(total);
+    n_kept = (int)block_sum64((u64)n_kept);
 
     if (wave != 0) return;
     const double u = a.u[row];
@@ -401,8 +496,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
                 a.id[row] = i0 + e;
                 if (a.p) a.p[row] = (float)((double)w[e] / (double)total);
                 if (a.logprob) {
-                    const double d = ((double)x[e] - wt.max) * c * 0.693147180559945309417;
-                    const double z0 = by_k || by_p || by_m ? whole : (double)total / wt.one;
+                    const double d = ((double)x[e] - (double)top) * c * 0.693147180559945309417;
+                    const double z0 = by_k || by_p || by_m ? whole : (double)total / one;
                     a.logprob[row] = (float)(d - log(z0));
                 }
                 if (a.n_kept) a.n_kept[row] = n_kept;
@@ -418,17 +513,22 @@ void launch_sample_rows(const ss_sample_rows_args& a, hipStream_t st) {
     int bits = 0;
     while ((1 << bits) < a.n_vocab) bits++;
     const int S = std::min(51, 62 - bits);
-    auto go = [&](auto t) {
+    auto go = [&](auto t, auto threads) {
         typedef decltype(t) T;
+        constexpr int TH = threads.value;
         const int groups = (a.n_vocab + Row<T>::GROUP - 1) / Row<T>::GROUP;
-        constexpr int most = (1 << 20) / Row<T>::GROUP * 8;               // beside ~35 KB of static LDS
+        constexpr int most = (1 << 20) / Row<T>::GROUP * 8;               // beside ~51 KB of static LDS
         static std::atomic<uint64_t> once{0};
-        once_per_device(once, [&] { SS_HIP(hipFuncSetAttribute((const void*)sample_rows_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, most)); });
-        sample_rows_kernel<T><<<a.n_rows, kThreads, (size_t)groups * 8, st>>>(a, S);
+        once_per_device(once, [&] { SS_HIP(hipFuncSetAttribute((const void*)sample_rows_kernel<T, TH>, hipFuncAttributeMaxDynamicSharedMemorySize, most)); });
+        sample_rows_kernel<T, TH><<<a.n_rows, TH, (size_t)groups * 8, st>>>(a, S);
     };
-    if (a.dtype == SS_DTYPE_F32) go(0.0f);
-    else if (a.dtype == SS_DTYPE_F16) go(f16());
-    else go(bf16());
+    auto by_rows = [&](auto t) {
+        if (a.n_rows <= 256) go(t, std::integral_constant<int, 1024>());
+        else go(t, std::integral_constant<int, 512>());
+    };
+    if (a.dtype == SS_DTYPE_F32) by_rows(0.0f);
+    else if (a.dtype == SS_DTYPE_F16) by_rows(f16());
+    else by_rows(bf16());
     SS_LAUNCH_CHECK();
 }
 
