@@ -590,7 +590,7 @@ const char* bad_rows(const ss_kv_rows* r, int n_tokens, int heads, int dim, bool
 }
 const char* bad_heads(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads) {
     if (n_heads <= 0 || n_heads % c.n_kv_heads || n_heads > 1 << 16) return "n_heads must be a multiple of n_kv_heads (at most 65536)";
-    if ((int64_t)b.max_new * (n_heads / c.n_kv_heads) >= (int64_t)1 << 30 || (int64_t)b.n_tokens * n_heads >= (int64_t)1 << 32) return "too many query rows";
+    if ((int64_t)b.max_new * (n_heads / c.n_kv_heads) >= (int64_t)1 << 30 || (int64_t)b.n_tokens * n_heads >= (int64_t)1 << 31) return "too many query rows";
     // workgroups of either kernel (at most 64 key ranges each)
     if ((int64_t)b.n_seqs * c.n_kv_heads * (((int64_t)b.max_new * (n_heads / c.n_kv_heads) + 63) / 64) >= (int64_t)1 << 24) return "too many sequences x heads x query tiles";
     return nullptr;

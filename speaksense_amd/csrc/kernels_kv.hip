@@ -24,6 +24,9 @@ template <int D> constexpr int kKeyPitch = 2 * D + 16;
 template <int D> constexpr int kValuePitch = 2 * D + 32;
 template <int D> constexpr int kTileBuf = 64 * (kKeyPitch<D> + kValuePitch<D>) + 528;   // + 64 key scales, 64 relative value scales, sref, its move
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
 enum { K_F16 = 0, K_BF16 = 1, K_E4M3 = 2, K_I8 = 3 };   // what the cache holds
 
 struct KvArgs {
@@ -69,115 +72,157 @@ __device__ __forceinline__ int find_seq(const int* qs, int n_seqs, int t) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// append / read: one workgroup per token row and 256 / (head_dim / 8) of its 2 H key and value rows; 8 elements (16 bytes) a lane.
-// Bound by HBM: 2 bytes of tokens and 1 or 2 of codes per element, once each.
+// append / read.  A workgroup looks up where `per` consecutive token rows lie (one lane each, into LDS), then its threads run over their per x 2 H key and value
+// rows, 16 elements a lane.  Bound by HBM: 2 bytes of tokens and 1 or 2 of codes per element, once each; looking up costs four dependent loads, so a
+// workgroup takes several rows as soon as there are enough to fill the card (kv_rows_per_group).
 // ---------------------------------------------------------------------------------------------
+constexpr int kMostRows = 16;      // token rows of a workgroup
+
+// place[i] of token row t0 + i: its row of the cache (page * page_size + row in page), -1 on no page, -2 of no sequence
+__device__ __forceinline__ void find_places(const KvArgs& a, int t0, int per, long* place) {
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x, t = t0 + lane;
+        int s = find_seq(a.q_start, a.n_seqs, t0);
+        if (lane < per) {
+            long at = -2;
+            if (t < a.n_tokens) {
+                s = max(s, 0);
+                while (s < a.n_seqs && a.q_start[s + 1] <= t) s++;       // from the first row's sequence on
+                if (s < a.n_seqs) {
+                    const Span sp = seq_span(a, s);
+                    if (t >= sp.q0 && t < sp.q0 + sp.n_new) {
+                        const int pos = sp.pos0 + (t - sp.q0), page = pos < 0 ? -1 : page_at(a, s, pos >> a.page_shift);
+                        at = page < 0 ? -1 : ((long)page << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+                    }
+                }
+            }
+            place[lane] = at;
+        }
+    }
+    __syncthreads();
+}
 template <int LPR> __device__ __forceinline__ unsigned lanes_umax(unsigned v) {   // over the LPR lanes of a row
 #define SS_DPP_UMAX(CTRL) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false))
-    SS_DPP_UMAX(kDppXor1); SS_DPP_UMAX(kDppXor2); SS_DPP_UMAX(kDppHalfMirror);
-    if (LPR == 16) SS_DPP_UMAX(kDppRor8);
+    SS_DPP_UMAX(kDppXor1); SS_DPP_UMAX(kDppXor2);
+    if (LPR == 8) SS_DPP_UMAX(kDppHalfMirror);
 #undef SS_DPP_UMAX
     return v;
 }
-
-template <typename T, int KIND, int D>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, const T* __restrict__ kn, long k_row, long k_head, const T* __restrict__ vn, long v_row, long v_head) {
-    typedef typename Mfma<T>::V8 V8;
-    constexpr int LPR = D / 8;
-    const int t = blockIdx.x;
-    const int s = find_seq(a.q_start, a.n_seqs, t);
-    if (s < 0 || s >= a.n_seqs) return;                  // rows behind the last sequence
-    const Span sp = seq_span(a, s);
-    if (t < sp.q0 || t >= sp.q0 + sp.n_new) return;
-    const int pos = sp.pos0 + (t - sp.q0);
-    if (pos < 0) return;
-    const int page = page_at(a, s, pos >> a.page_shift);
-    if (page < 0) return;
-    const int item = blockIdx.y * 256 + threadIdx.x, r = item / LPR, c = item % LPR;
-    if (r >= 2 * a.H) return;
-    const bool is_v = r >= a.H;
-    const int h = is_v ? r - a.H : r;
-    const T* src = is_v ? vn + (long)t * v_row + (long)h * v_head : kn + (long)t * k_row + (long)h * k_head;
-    const V8 x = *(const V8*)(src + c * 8);
-    const long slot = ((long)h << a.page_shift) + (pos & ((1 << a.page_shift) - 1));   // row inside the page
-    char* dst = page_ptr(is_v ? a.v : a.k, page, a.page_bytes);
-    if constexpr (KIND == K_F16 || KIND == K_BF16) {
-        *(V8*)(dst + (slot * D + c * 8) * 2) = x;
-    } else {
-        float f[8];
-        unsigned top = 0;      // the largest magnitude as bits: a NaN outranks every number, so a row that holds one reads back as NaN
-#pragma unroll
-        for (int i = 0; i < 8; i++) { f[i] = (float)x[i]; top = max(top, __float_as_uint(f[i]) & 0x7fffffffu); }
-        top = lanes_umax<LPR>(top);
-        uint2 code;
-        char* sc = is_v ? a.vs : a.ks;
-        const long at = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
-        if constexpr (KIND == K_E4M3) {
-            const int e = e8m0_for_amax(__uint_as_float(top));
-            const float m = pow2_neg_of_e8m0(e);
-            code.x = pack_e4m3x4(f[0] * m, f[1] * m, f[2] * m, f[3] * m);
-            code.y = pack_e4m3x4(f[4] * m, f[5] * m, f[6] * m, f[7] * m);
-            if (c == 0) sc[at] = (char)e;
-        } else {
-            const float s8 = __uint_as_float(top) / 127.0f, by = s8 > 0.0f ? s8 : 1.0f;
-            unsigned b[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) b[i] = (unsigned)(int)fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f) & 0xffu;
-            code.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-            code.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
-            if (c == 0) ((float*)sc)[at] = s8;
-        }
-        *(uint2*)(dst + slot * D + c * 8) = code;
+// item -> (key or value head, token row, 16 elements), the elements first and the heads last: a head's rows of neighbouring positions touch in a page, so
+// neighbouring lanes read or write whole lines of it (with the tokens last: 64-byte pieces, the read of 32 windows 104 us instead of 93)
+template <int D> struct Item {
+    static constexpr int LPR = D / 16;
+    int i, h, c;                   // token row of the workgroup, head, piece of 16 elements
+    bool is_v;
+    __device__ __forceinline__ Item(int item, int shift, int H) {
+        const int r = item / LPR;
+        c = item % LPR;
+        i = r & ((1 << shift) - 1);
+        h = r >> shift;
+        is_v = h >= H;
+        if (is_v) h -= H;
     }
-}
-
+};
 __device__ __forceinline__ float i8_at(unsigned w, int i) { return (float)(int)(signed char)(w >> (8 * i)); }
 
 template <typename T, int KIND, int D>
-__global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, T* __restrict__ ko, long k_row, long k_head, T* __restrict__ vo, long v_row, long v_head) {
+__global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int shift, const T* __restrict__ kn, long k_row, long k_head, const T* __restrict__ vn, long v_row, long v_head) {
     typedef typename Mfma<T>::V8 V8;
-    constexpr int LPR = D / 8;
-    const int t = blockIdx.x;
-    const int s = find_seq(a.q_start, a.n_seqs, t);
-    if (s < 0 || s >= a.n_seqs) return;
-    const Span sp = seq_span(a, s);
-    if (t < sp.q0 || t >= sp.q0 + sp.n_new) return;
-    const int pos = sp.pos0 + (t - sp.q0);
-    const int page = pos < 0 ? -1 : page_at(a, s, pos >> a.page_shift);
-    const int item = blockIdx.y * 256 + threadIdx.x, r = item / LPR, c = item % LPR;
-    if (r >= 2 * a.H) return;
-    const bool is_v = r >= a.H;
-    const int h = is_v ? r - a.H : r;
-    V8 x;
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (T)0.0f;
-    if (page >= 0) {
-        const long slot = ((long)h << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
-        const char* src = page_ptr(is_v ? a.v : a.k, page, a.page_bytes);
+    __shared__ long place[kMostRows];
+    const int t0 = blockIdx.x << shift;
+    find_places(a, t0, 1 << shift, place);
+    const int items = (2 * a.H * Item<D>::LPR) << shift, mask = (1 << a.page_shift) - 1;
+    for (int item = blockIdx.y * 256 + threadIdx.x; item < items; item += gridDim.y * 256) {
+        const Item<D> it(item, shift, a.H);
+        const long at = place[it.i];
+        if (at < 0) continue;                            // the lanes of a row agree
+        const int t = t0 + it.i;
+        const T* src = (it.is_v ? vn + (long)t * v_row + (long)it.h * v_head : kn + (long)t * k_row + (long)it.h * k_head) + it.c * 16;
+        const V8 x[2] = {*(const V8*)src, *(const V8*)(src + 8)};
+        const int page = (int)(at >> a.page_shift);
+        const long slot = ((long)it.h << a.page_shift) + (at & mask);            // row inside the page
+        char* dst = page_ptr(it.is_v ? a.v : a.k, page, a.page_bytes);
         if constexpr (KIND == K_F16 || KIND == K_BF16) {
-            x = *(const V8*)(src + (slot * D + c * 8) * 2);
+            *(V8*)(dst + (slot * D + it.c * 16) * 2) = x[0];
+            *(V8*)(dst + (slot * D + it.c * 16 + 8) * 2) = x[1];
         } else {
-            const uint2 code = *(const uint2*)(src + slot * D + c * 8);
-            const char* sc = is_v ? a.vs : a.ks;
-            const long at = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
-            float f[8], m;
+            float f[16];
+            unsigned top = 0;      // the largest magnitude as bits: a NaN outranks every number, so a row that holds one reads back as NaN
+#pragma unroll
+            for (int i = 0; i < 16; i++) { f[i] = (float)x[i >> 3][i & 7]; top = max(top, __float_as_uint(f[i]) & 0x7fffffffu); }
+            top = lanes_umax<D / 16>(top);
+            u32x4 code;
+            char* sc = it.is_v ? a.vs : a.ks;
+            const long sat = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
             if constexpr (KIND == K_E4M3) {
-                m = __uint_as_float((unsigned)(unsigned char)sc[at] << 23);
-#define SS_F8(I, W, B) f[I] = __builtin_amdgcn_cvt_f32_fp8(W, B)
-                SS_F8(0, code.x, 0); SS_F8(1, code.x, 1); SS_F8(2, code.x, 2); SS_F8(3, code.x, 3);
-                SS_F8(4, code.y, 0); SS_F8(5, code.y, 1); SS_F8(6, code.y, 2); SS_F8(7, code.y, 3);
-#undef SS_F8
+                const int e = e8m0_for_amax(__uint_as_float(top));
+                const float m = pow2_neg_of_e8m0(e);
+#pragma unroll
+                for (int i = 0; i < 4; i++) code[i] = pack_e4m3x4(f[4 * i] * m, f[4 * i + 1] * m, f[4 * i + 2] * m, f[4 * i + 3] * m);
+                if (it.c == 0) sc[sat] = (char)e;
             } else {
-                m = ((const float*)sc)[at];
+                const float s8 = __uint_as_float(top) / 127.0f, by = s8 > 0.0f ? s8 : 1.0f;
+                unsigned b[16];
 #pragma unroll
-                for (int i = 0; i < 4; i++) { f[i] = i8_at(code.x, i); f[4 + i] = i8_at(code.y, i); }
+                for (int i = 0; i < 16; i++) b[i] = (unsigned)(int)fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f) & 0xffu;
+#pragma unroll
+                for (int i = 0; i < 4; i++) code[i] = b[4 * i] | b[4 * i + 1] << 8 | b[4 * i + 2] << 16 | b[4 * i + 3] << 24;
+                if (it.c == 0) ((float*)sc)[sat] = s8;
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = (T)(f[i] * m);
+            *(u32x4*)(dst + slot * D + it.c * 16) = code;
         }
     }
-    T* dst = is_v ? vo + (long)t * v_row + (long)h * v_head : ko + (long)t * k_row + (long)h * k_head;
-    *(V8*)(dst + c * 8) = x;
+}
+
+template <typename T, int KIND, int D>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, int shift, T* __restrict__ ko, long k_row, long k_head, T* __restrict__ vo, long v_row, long v_head) {
+    typedef typename Mfma<T>::V8 V8;
+    __shared__ long place[kMostRows];
+    const int t0 = blockIdx.x << shift;
+    find_places(a, t0, 1 << shift, place);
+    const int items = (2 * a.H * Item<D>::LPR) << shift, mask = (1 << a.page_shift) - 1;
+#pragma unroll 4
+    for (int item = blockIdx.y * 256 + threadIdx.x; item < items; item += gridDim.y * 256) {
+        const Item<D> it(item, shift, a.H);
+        const long at = place[it.i];
+        if (at == -2) continue;
+        V8 x[2];
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i >> 3][i & 7] = (T)0.0f;
+        if (at >= 0) {
+            const int page = (int)(at >> a.page_shift);
+            const long slot = ((long)it.h << a.page_shift) + (at & mask);
+            const char* src = page_ptr(it.is_v ? a.v : a.k, page, a.page_bytes);
+            if constexpr (KIND == K_F16 || KIND == K_BF16) {
+                x[0] = *(const V8*)(src + (slot * D + it.c * 16) * 2);
+                x[1] = *(const V8*)(src + (slot * D + it.c * 16 + 8) * 2);
+            } else {
+                const u32x4 code = *(const u32x4*)(src + slot * D + it.c * 16);
+                const char* sc = it.is_v ? a.vs : a.ks;
+                const long sat = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
+                float m;
+                if constexpr (KIND == K_E4M3) m = __uint_as_float((unsigned)(unsigned char)sc[sat] << 23);
+                else m = ((const float*)sc)[sat];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float f[4];
+                    if constexpr (KIND == K_E4M3) {
+                        f[0] = __builtin_amdgcn_cvt_f32_fp8(code[i], 0); f[1] = __builtin_amdgcn_cvt_f32_fp8(code[i], 1);
+                        f[2] = __builtin_amdgcn_cvt_f32_fp8(code[i], 2); f[3] = __builtin_amdgcn_cvt_f32_fp8(code[i], 3);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) f[e] = i8_at(code[i], e);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[i >> 1][4 * (i & 1) + e] = (T)(f[e] * m);
+                }
+            }
+        }
+        const int t = t0 + it.i;
+        T* dst = (it.is_v ? vo + (long)t * v_row + (long)it.h * v_head : ko + (long)t * k_row + (long)it.h * k_head) + it.c * 16;
+        *(V8*)dst = x[0];
+        *(V8*)(dst + 8) = x[1];
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -216,8 +261,6 @@ template <> struct Held<K_BF16> { typedef bf16 M; static constexpr int B = 2; };
 template <> struct Held<K_E4M3> { typedef f16 M; static constexpr int B = 1; };
 template <> struct Held<K_I8> { typedef f16 M; static constexpr int B = 1; };
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ unsigned perm(unsigned hi, unsigned lo, unsigned sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
 
 // four codes -> two f16 pairs.  int8: byte u = code + 128 under the byte 0x64 is the f16 number 1024 + u; minus 1152 gives the code, exactly
@@ -896,12 +939,14 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     }
 }
 
-// one wave per query row: join its key ranges.  `few`: rows of the few-row kernel (n_new G <= 16), else those of the tile kernel (`all`: every row)
+// One workgroup per query row joins its key ranges: 4 waves take them in turn, 8 loads in flight each.  `few`: rows of the few-row kernel (n_new G <= 16),
+// else those of the tile kernel (`all`: every row).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t, int few) {
-    const int heads = a.H * t.G, lane = threadIdx.x & 63;
-    const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (long)a.n_tokens * heads) return;
+    constexpr int E = D / 64;
+    __shared__ float s_acc[4][D];
+    const int heads = a.H * t.G, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long at = blockIdx.x;
     const int row = (int)(at / heads), head = (int)(at % heads);
     const int s = find_seq(a.q_start, a.n_seqs, row);
     if (s < 0 || s >= a.n_seqs) return;
@@ -911,22 +956,31 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t,
     const float2 ml = lane < t.splits ? t.part_ml[at * t.splits + lane] : make_float2(-kInf, 0.0f);
     const float m = wave_max(ml.x), f = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
     const float L = wave_sum(ml.y * f);
-    constexpr int E = D / 64;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = 0.0f;
-    for (int i = 0; i < t.splits; i++) {
-        const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), i));
-        if (w == 0.0f) continue;
-        const float* o = t.part + (at * t.splits + i) * D + lane * E;
+    for (int i0 = wave * 8; i0 < t.splits; i0 += 32) {
+        float o[8][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) acc[e] += w * o[e];
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < E; e++) o[i][e] = t.part[(at * t.splits + min(i0 + i, t.splits - 1)) * D + lane * E + e];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {                      // beyond the last range the weight is 0
+            const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(i0 + i, 63)));
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e] += i0 + i < t.splits ? w * o[i][e] : 0.0f;
+        }
     }
-    const float inv = L > 0.0f ? 1.0f / L : L;
-    T* o = (T*)t.out + (long)row * t.o_row + (long)head * t.o_head + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = (T)(acc[e] * inv);
-    if (t.lse && lane == 0) t.lse[at] = L > 0.0f ? (m + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
+    for (int e = 0; e < E; e++) s_acc[wave][lane * E + e] = acc[e];
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const int d = threadIdx.x;
+        const float inv = L > 0.0f ? 1.0f / L : L;
+        ((T*)t.out)[(long)row * t.o_row + (long)head * t.o_head + d] = (T)(((s_acc[0][d] + s_acc[1][d]) + (s_acc[2][d] + s_acc[3][d])) * inv);
+    }
+    if (t.lse && threadIdx.x == 0) t.lse[at] = L > 0.0f ? (m + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
 }
 
 KvArgs kv_args(const ss_kv_cache& c, const ss_kv_batch& b) {
@@ -954,25 +1008,41 @@ int up(long a, long b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
 
+// log2 of the token rows of a workgroup, and workgroups side by side on them: enough workgroups to fill the card come first (small calls are all latency),
+// then rows
+static int kv_rows_per_group(const ss_kv_cache& c, const ss_kv_batch& b, int* side) {
+    int shift = 0;
+    while ((2 << shift) <= kMostRows && b.n_tokens >> (shift + 1) >= 512) shift++;
+    *side = std::max(1, (int)std::min((long)up(((2l * c.n_kv_heads * (c.head_dim / 16)) << shift), 256), 2048l / up(b.n_tokens, 1 << shift)));
+    return shift;
+}
+
 void launch_kv_append(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& k, const ss_kv_rows& v, hipStream_t st) {
     if (b.n_tokens == 0 || b.n_seqs == 0) return;
-    const dim3 grid(b.n_tokens, up(2l * c.n_kv_heads * (c.head_dim / 8), 256));
+    int side;
+    const int shift = kv_rows_per_group(c, b, &side);
     by_type(c, [&](auto t, auto kind, auto dim) {
         typedef decltype(t) T;
-        kv_append_kernel<T, kind.value, dim.value><<<grid, 256, 0, st>>>(kv_args(c, b), (const T*)k.p, k.row_stride, k.head_stride, (const T*)v.p, v.row_stride, v.head_stride);
+        kv_append_kernel<T, kind.value, dim.value><<<dim3(up(b.n_tokens, 1 << shift), side), 256, 0, st>>>(kv_args(c, b), shift, (const T*)k.p, k.row_stride, k.head_stride, (const T*)v.p,
+                                                                                                     v.row_stride, v.head_stride);
     });
     SS_LAUNCH_CHECK();
 }
 
 void launch_kv_read(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& k, const ss_kv_rows& v, hipStream_t st) {
     if (b.n_tokens == 0 || b.n_seqs == 0) return;
-    const dim3 grid(b.n_tokens, up(2l * c.n_kv_heads * (c.head_dim / 8), 256));
+    int side;
+    const int shift = kv_rows_per_group(c, b, &side);
     by_type(c, [&](auto t, auto kind, auto dim) {
         typedef decltype(t) T;
-        kv_read_kernel<T, kind.value, dim.value><<<grid, 256, 0, st>>>(kv_args(c, b), (T*)k.p, k.row_stride, k.head_stride, (T*)v.p, v.row_stride, v.head_stride);
+        kv_read_kernel<T, kind.value, dim.value><<<dim3(up(b.n_tokens, 1 << shift), side), 256, 0, st>>>(kv_args(c, b), shift, (T*)k.p, k.row_stride, k.head_stride, (T*)v.p,
+                                                                                                   v.row_stride, v.head_stride);
     });
     SS_LAUNCH_CHECK();
 }
+
+// Up to so many keys a batch that mixes chunks with short spans runs on the tile kernel alone
+constexpr long kTileTakesAll = 2048;
 
 KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads) {
     KvPlan p{};
@@ -982,7 +1052,7 @@ KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads
     const long cap = (long)b.max_pages * c.page_size, keys = std::max(1l, b.max_len > 0 ? std::min((long)b.max_len, cap) : cap);
     const long rows = (long)b.max_new * G, pairs = (long)b.n_seqs * c.n_kv_heads;
     p.tile = rows > 16;
-    p.few = !p.tile || (long)std::max(b.min_new, 1) * G <= 16;
+    p.few = !p.tile || ((long)std::max(b.min_new, 1) * G <= 16 && keys > kTileTakesAll);
     p.qc = rows <= 64 ? 1 : rows < 1024 || c.head_dim == 128 ? 2 : 4;
     p.few_keys = p.tile_keys = (int)std::min(keys, 1l << 30);
     auto cut = [&](long groups, long want, int least, int* splits, int* len) {   // as many key ranges as fill the card, none shorter than `least`
@@ -1012,7 +1082,7 @@ void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv
         constexpr int K = kind.value, D = dim.value;
         auto join = [&](int few) {
             if (t.splits == 1) return;
-            kv_attn_join_kernel<T, D><<<up((long)b.n_tokens * n_heads, 4), 256, 0, st>>>(a, t, few);
+            kv_attn_join_kernel<T, D><<<(unsigned)((long)b.n_tokens * n_heads), 256, 0, st>>>(a, t, few);
             SS_LAUNCH_CHECK();
         };
         auto part = [&](int splits, int keys) {            // the two kernels follow each other on the stream: they may share the workspace
