@@ -73,7 +73,7 @@ __device__ __forceinline__ int find_seq(const int* qs, int n_seqs, int t) {
 
 // ---------------------------------------------------------------------------------------------
 // append / read.  A workgroup looks up where `per` consecutive token rows lie (one lane each, into LDS), then its threads run over their per x 2 H key and value
-// rows, 16 elements a lane.  Bound by HBM: 2 bytes of tokens and 1 or 2 of codes per element, once each; looking up costs four dependent loads, so a
+// rows, 16 (append) or 8 (read) elements a lane.  Bound by HBM: 2 bytes of tokens and 1 or 2 of codes per element, once each; looking up costs four dependent loads, so a
 // workgroup takes several rows as soon as there are enough to fill the card (kv_rows_per_group).
 // ---------------------------------------------------------------------------------------------
 constexpr int kMostRows = 16;      // token rows of a workgroup
@@ -108,11 +108,11 @@ template <int LPR> __device__ __forceinline__ unsigned lanes_umax(unsigned v) { 
 #undef SS_DPP_UMAX
     return v;
 }
-// item -> (key or value head, token row, 16 elements), the elements first and the heads last: a head's rows of neighbouring positions touch in a page, so
+// item -> (key or value head, token row, PER elements), the elements first and the heads last: a head's rows of neighbouring positions touch in a page, so
 // neighbouring lanes read or write whole lines of it (with the tokens last: 64-byte pieces, the read of 32 windows 104 us instead of 93)
-template <int D> struct Item {
-    static constexpr int LPR = D / 16;
-    int i, h, c;                   // token row of the workgroup, head, piece of 16 elements
+template <int D, int PER> struct Item {
+    static constexpr int LPR = D / PER;
+    int i, h, c;                   // token row of the workgroup, head, piece of PER elements
     bool is_v;
     __device__ __forceinline__ Item(int item, int shift, int H) {
         const int r = item / LPR;
@@ -131,9 +131,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int shift, con
     __shared__ long place[kMostRows];
     const int t0 = blockIdx.x << shift;
     find_places(a, t0, 1 << shift, place);
-    const int items = (2 * a.H * Item<D>::LPR) << shift, mask = (1 << a.page_shift) - 1;
+    const int items = (2 * a.H * Item<D, 16>::LPR) << shift, mask = (1 << a.page_shift) - 1;
     for (int item = blockIdx.y * 256 + threadIdx.x; item < items; item += gridDim.y * 256) {
-        const Item<D> it(item, shift, a.H);
+        const Item<D, 16> it(item, shift, a.H);
         const long at = place[it.i];
         if (at < 0) continue;                            // the lanes of a row agree
         const int t = t0 + it.i;
@@ -162,9 +162,25 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int shift, con
                 if (it.c == 0) sc[sat] = (char)e;
             } else {
                 const float s8 = __uint_as_float(top) / 127.0f, by = s8 > 0.0f ? s8 : 1.0f;
+                // x / s as IEEE rounds it (ties of the code depend on it, and of 16-bit rows one element in 400 lies on a tie): from the correctly rounded
+                // reciprocal of the row, two corrections by the exact remainder, 5 instructions an element instead of the division's 11
+                const float r = 1.0f / by;
+                float q[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float y = f[i] * r;
+                    y = fmaf(fmaf(-by, y, f[i]), r, y);
+                    y = fmaf(fmaf(-by, y, f[i]), r, y);
+                    q[i] = rintf(y);
+                }
+                if (__ballot(!(by > 1e-30f && by < 1e30f))) {    // remainders out of float's range; a NaN
+                    asm volatile("");
+#pragma unroll
+                    for (int i = 0; i < 16; i++) q[i] = fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f);
+                }
                 unsigned b[16];
 #pragma unroll
-                for (int i = 0; i < 16; i++) b[i] = (unsigned)(int)fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f) & 0xffu;
+                for (int i = 0; i < 16; i++) b[i] = (unsigned)(int)q[i] & 0xffu;
 #pragma unroll
                 for (int i = 0; i < 4; i++) code[i] = b[4 * i] | b[4 * i + 1] << 8 | b[4 * i + 2] << 16 | b[4 * i + 3] << 24;
                 if (it.c == 0) ((float*)sc)[sat] = s8;
@@ -174,37 +190,39 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int shift, con
     }
 }
 
-template <typename T, int KIND, int D>
+// NT: results of more than kNtBytes leave past the caches, which could not hold them for their reader anyway (245 MB: 64 instead of 83 us from 8 bits, 77
+// instead of 102 from 16; at 31 MB there is no difference, and the reader finds them cached).  8 elements a lane: each store instruction
+// writes whole lines (16, two stores each: 94 us).
+constexpr long kNtBytes = 128l << 20;
+template <typename T, int KIND, int D, bool NT>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, int shift, T* __restrict__ ko, long k_row, long k_head, T* __restrict__ vo, long v_row, long v_head) {
     typedef typename Mfma<T>::V8 V8;
     __shared__ long place[kMostRows];
     const int t0 = blockIdx.x << shift;
     find_places(a, t0, 1 << shift, place);
-    const int items = (2 * a.H * Item<D>::LPR) << shift, mask = (1 << a.page_shift) - 1;
+    const int items = (2 * a.H * Item<D, 8>::LPR) << shift, mask = (1 << a.page_shift) - 1;
 #pragma unroll 4
     for (int item = blockIdx.y * 256 + threadIdx.x; item < items; item += gridDim.y * 256) {
-        const Item<D> it(item, shift, a.H);
+        const Item<D, 8> it(item, shift, a.H);
         const long at = place[it.i];
         if (at == -2) continue;
-        V8 x[2];
+        V8 x;
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i >> 3][i & 7] = (T)0.0f;
+        for (int i = 0; i < 8; i++) x[i] = (T)0.0f;
         if (at >= 0) {
             const int page = (int)(at >> a.page_shift);
             const long slot = ((long)it.h << a.page_shift) + (at & mask);
             const char* src = page_ptr(it.is_v ? a.v : a.k, page, a.page_bytes);
-            if constexpr (KIND == K_F16 || KIND == K_BF16) {
-                x[0] = *(const V8*)(src + (slot * D + it.c * 16) * 2);
-                x[1] = *(const V8*)(src + (slot * D + it.c * 16 + 8) * 2);
-            } else {
-                const u32x4 code = *(const u32x4*)(src + slot * D + it.c * 16);
+            if constexpr (KIND == K_F16 || KIND == K_BF16) x = *(const V8*)(src + (slot * D + it.c * 8) * 2);
+            else {
+                const u32x2 code = *(const u32x2*)(src + slot * D + it.c * 8);
                 const char* sc = it.is_v ? a.vs : a.ks;
                 const long sat = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
                 float m;
                 if constexpr (KIND == K_E4M3) m = __uint_as_float((unsigned)(unsigned char)sc[sat] << 23);
                 else m = ((const float*)sc)[sat];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
+                for (int i = 0; i < 2; i++) {
                     float f[4];
                     if constexpr (KIND == K_E4M3) {
                         f[0] = __builtin_amdgcn_cvt_f32_fp8(code[i], 0); f[1] = __builtin_amdgcn_cvt_f32_fp8(code[i], 1);
@@ -214,14 +232,14 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, int shift, T* __
                         for (int e = 0; e < 4; e++) f[e] = i8_at(code[i], e);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[i >> 1][4 * (i & 1) + e] = (T)(f[e] * m);
+                    for (int e = 0; e < 4; e++) x[4 * i + e] = (T)(f[e] * m);
                 }
             }
         }
         const int t = t0 + it.i;
-        T* dst = (it.is_v ? vo + (long)t * v_row + (long)it.h * v_head : ko + (long)t * k_row + (long)it.h * k_head) + it.c * 16;
-        *(V8*)dst = x[0];
-        *(V8*)(dst + 8) = x[1];
+        T* dst = (it.is_v ? vo + (long)t * v_row + (long)it.h * v_head : ko + (long)t * k_row + (long)it.h * k_head) + it.c * 8;
+        if constexpr (NT) __builtin_nontemporal_store(x, (V8*)dst);
+        else *(V8*)dst = x;
     }
 }
 
@@ -1010,17 +1028,17 @@ int up(long a, long b) { return (int)((a + b - 1) / b); }
 
 // log2 of the token rows of a workgroup, and workgroups side by side on them: enough workgroups to fill the card come first (small calls are all latency),
 // then rows
-static int kv_rows_per_group(const ss_kv_cache& c, const ss_kv_batch& b, int* side) {
+static int kv_rows_per_group(const ss_kv_cache& c, const ss_kv_batch& b, int elements, int* side) {
     int shift = 0;
     while ((2 << shift) <= kMostRows && b.n_tokens >> (shift + 1) >= 512) shift++;
-    *side = std::max(1, (int)std::min((long)up(((2l * c.n_kv_heads * (c.head_dim / 16)) << shift), 256), 2048l / up(b.n_tokens, 1 << shift)));
+    *side = std::max(1, (int)std::min((long)up((2l * c.n_kv_heads * (c.head_dim / elements)) << shift, 256), 2048l / up(b.n_tokens, 1 << shift)));
     return shift;
 }
 
 void launch_kv_append(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& k, const ss_kv_rows& v, hipStream_t st) {
     if (b.n_tokens == 0 || b.n_seqs == 0) return;
     int side;
-    const int shift = kv_rows_per_group(c, b, &side);
+    const int shift = kv_rows_per_group(c, b, 16, &side);
     by_type(c, [&](auto t, auto kind, auto dim) {
         typedef decltype(t) T;
         kv_append_kernel<T, kind.value, dim.value><<<dim3(up(b.n_tokens, 1 << shift), side), 256, 0, st>>>(kv_args(c, b), shift, (const T*)k.p, k.row_stride, k.head_stride, (const T*)v.p,
@@ -1032,11 +1050,15 @@ void launch_kv_append(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_ro
 void launch_kv_read(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows& k, const ss_kv_rows& v, hipStream_t st) {
     if (b.n_tokens == 0 || b.n_seqs == 0) return;
     int side;
-    const int shift = kv_rows_per_group(c, b, &side);
+    const int shift = kv_rows_per_group(c, b, 8, &side);
     by_type(c, [&](auto t, auto kind, auto dim) {
         typedef decltype(t) T;
-        kv_read_kernel<T, kind.value, dim.value><<<dim3(up(b.n_tokens, 1 << shift), side), 256, 0, st>>>(kv_args(c, b), shift, (T*)k.p, k.row_stride, k.head_stride, (T*)v.p,
-                                                                                                   v.row_stride, v.head_stride);
+        auto go = [&](auto nt) {
+            kv_read_kernel<T, kind.value, dim.value, nt.value><<<dim3(up(b.n_tokens, 1 << shift), side), 256, 0, st>>>(kv_args(c, b), shift, (T*)k.p, k.row_stride, k.head_stride,
+                                                                                                                       (T*)v.p, v.row_stride, v.head_stride);
+        };
+        if (4l * b.n_tokens * c.n_kv_heads * c.head_dim > kNtBytes) go(std::true_type());
+        else go(std::false_type());
     });
     SS_LAUNCH_CHECK();
 }
