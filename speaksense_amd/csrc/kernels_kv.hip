@@ -532,8 +532,9 @@ template <int KIND, int D> struct KvTile {
     }
 };
 
+// (launch bounds: head_dim 64 at 3 waves a SIMD, 76 us for 96 windows; at 4 it spills, 103)
 template <typename T, int KIND, int D>
-__global__ __launch_bounds__(256) void kv_attn_few_kernel(KvArgs a, AttnArgs t) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArgs a, AttnArgs t) {
     typedef typename Held<KIND>::M M;
     typedef typename Mfma<M>::V8 V8;
     constexpr bool SCALED = Held<KIND>::B == 1;
@@ -1082,7 +1083,7 @@ KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads
         *len = (int)((keys + n * 128 - 1) / (n * 128) * 128);
         *splits = (int)((keys + *len - 1) / *len);
     };
-    if (p.few) cut(pairs, 1024, 256, &p.few_splits, &p.few_keys);
+    if (p.few) cut(pairs, 512, 512, &p.few_splits, &p.few_keys);
     if (p.tile) cut(pairs * up(rows, 64 * p.qc), 512, 512, &p.tile_splits, &p.tile_keys);
     const int n = std::max(p.few_splits, p.tile_splits);
     if (n > 1) p.workspace = (int64_t)b.n_tokens * n_heads * n * (c.head_dim + 2) * 4;
