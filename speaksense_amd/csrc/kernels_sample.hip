@@ -2,8 +2,8 @@
 //
 // With max = the row's largest logit and c = log2(e) / t, id i weighs 2^((x_i - max) c), held as an integer W_i = round(w_i 2^S), S = 62 - ceil(log2 n_vocab)
 // (at most 51): every sum of a row fits 62 bits and is exact, so neither the order of the atomics nor the split over waves can change a result, and a running
-// sum is compared with u times the total exactly.  The exponential is evaluated in double: 2^y = 2^(k/256) 2^r, k = round(256 y), |r| <= 1/512, the first
-// factor from a table, the second from its series up to r^3 (the next term is below 1.4e-13 of it).
+// sum is compared with u times the total exactly.  The exponential is evaluated in double: 2^y = 2^(k/1024) 2^r, k = round(1024 y), |r| <= 1/2048, the
+// first factor from a table, the second from its series up to r^2 (the next term is below 7e-12 of it).
 //
 // top-k and top-p are both "keep an id while the measure of the better ones stays below a target", the measure being 1 or W: a histogram over
 // 2048 equal steps of the logit finds the step in which the target is crossed, the ids of that step are gathered into LDS and ranked there exactly by
@@ -34,11 +34,6 @@ template <typename T> struct Row {
     typedef T V __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
     const T* p;
     int n, groups;
-    bool inf_row;                  // the largest logit is +inf: only those ids count, all alike
-    __device__ __forceinline__ float clean(T v) const {
-        const float x = fmaxf((float)v, -kInf);          // NaN counts as masked
-        return inf_row ? (x == kInf ? 0.0f : -kInf) : x;
-    }
     // this lane's VEC consecutive ids of group g, as they lie in memory; a lane that the row's end cuts reads nothing here
     __device__ __forceinline__ V fetch(int g, int lane) const {
         const int i0 = g * GROUP + lane * VEC;
@@ -46,15 +41,15 @@ template <typename T> struct Row {
         if (i0 + VEC <= n) v = *(const V*)(p + i0);
         return v;
     }
-    // their values x[]; ids behind the row are masked; returns the first id
+    // their values x[], NaN as it is; ids behind the row are masked; returns the first id
     __device__ __forceinline__ int values(int g, int lane, V v, float* x) const {
         const int i0 = g * GROUP + lane * VEC;
         if (i0 + VEC <= n) {
 #pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = clean(v[e]);
+            for (int e = 0; e < VEC; e++) x[e] = (float)v[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = i0 + e < n ? clean(p[i0 + e]) : -kInf;
+            for (int e = 0; e < VEC; e++) x[e] = i0 + e < n ? (float)p[i0 + e] : -kInf;
         }
         return i0;
     }
@@ -62,18 +57,18 @@ template <typename T> struct Row {
 };
 
 struct Weight {                    // w(x) 2^S in double and as an integer
-    const double* table;           // LDS: 2^(j/256 + S)
+    const double* table;           // LDS: 2^(j/1024 + S)
     double top, c, least;          // y = (x - top) c; below `least` w 2^S is less than 2^-16 and counts as that, which rounds to 0
     __device__ __forceinline__ double scaled(float x) const {
         const double y = fmax(((double)x - top) * c, least);
-        constexpr double magic = 6755399441055744.0 / 256.0;             // 1.5 2^52 / 256: adding it rounds y to a multiple of 1/256
+        constexpr double magic = 6755399441055744.0 / 1024.0;            // 1.5 2^52 / 1024: adding it rounds y to a multiple of 1/1024
         const double z = y + magic;
-        const int k = (int)(unsigned)__double_as_longlong(z);            // low word of the mantissa: 256 y, rounded, two's complement
+        const int k = (int)(unsigned)__double_as_longlong(z);            // low word of the mantissa: 1024 y, rounded, two's complement
         const double r = y - (z - magic);
-        constexpr double L1 = 0.693147180559945309417, L2 = 0.240226506959100712333, L3 = 0.0555041086648215799532;
-        const double q = r * fma(r, fma(r, L3, L2), L1);
-        const double t = table[k & 255];
-        const double s = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));   // the exponent: -16 <= k / 256 + S <= 51
+        constexpr double L1 = 0.693147180559945309417, L2 = 0.240226506959100712333;
+        const double q = r * fma(r, L2, L1);
+        const double t = table[k & 1023];
+        const double s = __hiloint2double(__double2hiint(t) + ((k >> 10) << 20), __double2loint(t));  // the exponent: -16 <= k / 1024 + S <= 51
         return fma(s, q, s);
     }
     static __device__ __forceinline__ u64 integer(double s) {            // round(s), 0 <= s <= 2^51
@@ -107,16 +102,15 @@ __device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {            // incl
 }
 
 template <int THREADS> struct Shared {
-    double table[256];
+    double table[1024];
     u64 hist[kBins];
     Entry list[kList];             // the ids of the step in which a target is crossed
-    Entry kept[kList];             // the ids above it, and of it those that stay: everything that is kept, if it fits
+    Entry kept[kList];             // the ids of that step and of the better ones, if they fit
     u64 wave64[THREADS / 64 + 1];
     float wave_f[2][THREADS / 64];
-    int wave_i[THREADS / 64];
     u64 found_base;
     unsigned found_key, key_lo, key_hi;
-    int found, found_id, n_list, n_kept;
+    int found, found_id, n_list, n_kept, best;
 };
 
 template <typename T, int THREADS>
@@ -128,7 +122,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
     typedef Row<T> R;
     constexpr int VEC = R::VEC, AHEAD = 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
-    R r{(const T*)a.logits + (long)row * a.row_stride, a.n_vocab, (a.n_vocab + R::GROUP - 1) / R::GROUP, false};
+    R r{(const T*)a.logits + (long)row * a.row_stride, a.n_vocab, (a.n_vocab + R::GROUP - 1) / R::GROUP};
 
     // f(group, first id of the lane, its VEC logits) over the wave's groups, the loads of the next AHEAD groups in flight.  f appears once in a rolled
     // loop: a workgroup runs through its code only a few times, and instruction fetches cost more than the moves between the buffers.
@@ -147,33 +141,25 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
         }
     };
 
-    // the largest logit (lowest id), the smallest unmasked one
-    float top = -kInf, low = kInf;
-    int best = 0x7fffffff;
-    over_row([&](int, int i0, const float* x) {
+    // the largest logit; the smallest unmasked one of a sample (it only scales the histograms' steps)
+    float mine = -kInf, low = kInf;
+    over_row([&](int g, int, const float* x) {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            if (x[e] > top) { top = x[e]; best = i0 + e; }
-            low = fminf(low, x[e] > -kInf ? x[e] : kInf);
-        }
+        for (int e = 0; e < VEC; e++) mine = fmaxf(mine, x[e]);          // passes over NaN
+        if (g == wave)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) low = fminf(low, x[e] > -kInf ? x[e] : kInf);
     });
-    for (int i = tid; i < 256; i += THREADS) sh.table[i] = exp2(i * (1.0 / 256.0) + S);
+    for (int i = tid; i < 1024; i += THREADS) sh.table[i] = exp2(i * (1.0 / 1024.0) + S);
     {
-        const float wt = wave_max(top);
-        int wb = top == wt ? best : 0x7fffffff;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) wb = min(wb, __shfl_xor(wb, o));
-        const float wl = -wave_max(-low);
-        if (lane == 0) { sh.wave_f[0][wave] = wt; sh.wave_i[wave] = wb; sh.wave_f[1][wave] = wl; }
+        const float wt = wave_max(mine), wl = -wave_max(-low);
+        if (lane == 0) { sh.wave_f[0][wave] = wt; sh.wave_f[1][wave] = wl; }
+        if (tid == 0) sh.best = 0x7fffffff;
     }
     __syncthreads();
-    top = -kInf; best = 0x7fffffff; low = kInf;
-    for (int w = 0; w < WAVES; w++) {
-        const float t = sh.wave_f[0][w];
-        const int b = sh.wave_i[w];
-        if (t > top) { top = t; best = b; } else if (t == top) best = min(best, b);
-        low = fminf(low, sh.wave_f[1][w]);
-    }
+    float top = -kInf;
+    low = kInf;
+    for (int w = 0; w < WAVES; w++) { top = fmaxf(top, sh.wave_f[0][w]); low = fminf(low, sh.wave_f[1][w]); }
     if (top == -kInf) {                                                   // every id is masked
         if (tid == 0) {
             a.id[row] = -1;
@@ -183,7 +169,44 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
         }
         return;
     }
-    if (top == kInf) { r.inf_row = true; top = low = 0.0f; }
+    auto block_sum64 = [&](u64 v) {
+        v = wave_sum64(v);
+        __syncthreads();
+        if (lane == 0) sh.wave64[wave] = v;
+        __syncthreads();
+        u64 t = 0;
+        for (int w = 0; w < WAVES; w++) t += sh.wave64[w];
+        __syncthreads();
+        return t;
+    };
+    // one wave: the id at place `need` (from 1) among the ids that `is` says yes to, counted in order of id; mass[] holds their number in each group
+    auto nth = [&](u64 need, auto is) {
+        u64 run = 0;
+        int at = 0;
+        for (; at < r.groups - 1 && run + mass[at] < need; at++) run += mass[at];
+        float x[VEC];
+        const int i0 = r.load(at, lane, x);
+        u64 n = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) n += is(x[e], i0 + e);
+        const u64 inc = run + wave_scan64(n, lane);
+        if (inc - n < need && need <= inc) {
+            n = inc - n;
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (is(x[e], i0 + e) && ++n == need) sh.found_id = i0 + e;
+        }
+    };
+    auto count_groups = [&](auto is) {
+        over_row([&](int g, int i0, const float* x) {
+            u64 n = 0;
+#pragma unroll
+            for (int e = 0; e < VEC; e++) n += is(x[e], i0 + e);
+            n = wave_sum64(n);
+            if (lane == 0) mass[g] = n;
+        });
+        __syncthreads();
+    };
 
     const float t_row = a.temperature ? a.temperature[row] : 1.0f;
     const bool greedy = !(t_row > 0.0f);
@@ -202,15 +225,16 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
     // the sum of all weights, for logprob: of float32 exponentials where some pass goes over the whole row and needs no exact ones, else exact
     float part = 0.0f;
     double whole = 0.0;
+    bool summed = false;
     const float cf = (float)c;
     const bool plain = c > 1e-30 && c < 1e30;                             // float32 takes it
-    auto add_parts = [&](const float* x) {
+    auto add_parts = [&](const float* x) {                                // NaN counts as masked: fmaxf passes over it
         if (plain)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) part += __builtin_amdgcn_exp2f((x[e] - top) * cf);
+            for (int e = 0; e < VEC; e++) part += __builtin_amdgcn_exp2f(fmaxf((x[e] - top) * cf, -kInf));
         else
 #pragma unroll
-            for (int e = 0; e < VEC; e++) part += __builtin_amdgcn_exp2f((float)((double)(x[e] - top) * c));
+            for (int e = 0; e < VEC; e++) part += __builtin_amdgcn_exp2f(fmaxf((float)((double)(x[e] - top) * c), -kInf));
     };
     auto sum_parts = [&]() {
         const double s = (double)wave_sum(part);
@@ -221,89 +245,145 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
         for (int w = 0; w < WAVES; w++) whole += __longlong_as_double((long long)sh.wave64[w]);
         __syncthreads();
     };
-    if (greedy) {
-        if (a.logprob) {
-            over_row([&](int, int, const float* x) { add_parts(x); });
-            sum_parts();
+    if (top == kInf) {                                                    // ids at +inf share all weight, the others are masked
+        auto is = [&](float x, int) { return x == kInf; };
+        u64 n = 0;
+        count_groups(is);
+        for (int g = tid; g < r.groups; g += THREADS) n += mass[g];
+        n = block_sum64(n);
+        u64 m = greedy ? 1 : by_k ? min(n, (u64)k_row) : n;
+        if (by_p) m = max((u64)1, (u64)ceil((double)fmaxf(p_row, 0.0f) * (double)m));
+        if (wave == 0) {
+            const double u = a.u[row];
+            u64 j = !greedy && u > 0.0 ? (u64)fmin(u * (double)m, (double)m) : 0;
+            nth(min(j, m - 1) + 1, is);
+            if (lane == 0) {
+                a.id[row] = sh.found_id;
+                if (a.p) a.p[row] = (float)(1.0 / (double)m);
+                if (a.logprob) a.logprob[row] = (float)-log((double)n);
+                if (a.n_kept) a.n_kept[row] = (int)m;
+            }
         }
+        return;
+    }
+    if (greedy) {
+        over_row([&](int, int i0, const float* x) {
+            if (a.logprob) add_parts(x);
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (x[e] == top) atomicMin(&sh.best, i0 + e);
+        });
+        if (a.logprob) sum_parts();
+        __syncthreads();
         if (tid == 0) {
-            a.id[row] = best;
+            a.id[row] = sh.best;
             if (a.p) a.p[row] = 1.0f;
             if (a.logprob) a.logprob[row] = (float)-log(whole);
             if (a.n_kept) a.n_kept[row] = 1;
         }
         return;
     }
-    __syncthreads();                                                      // the table
 
     float thr = -kInf;                                                    // kept: x > thr, or x == thr and id <= thr_id
     int thr_id = -1;
     auto alive = [&](float x, int id) { return x > thr || (x == thr && id <= thr_id); };
     const float steps = low < top ? (float)(kBins - 1) / (top - low) : 0.0f;
-    auto bin_of = [&](float x) { return min((int)((top - x) * steps), kBins - 1); };
+    auto bin_of = [&](float x) { return (int)fminf(fmaxf((top - x) * steps, 0.0f), (float)(kBins - 1)); };   // NaN: 0
     auto value_of = [&](unsigned key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); };
 
-    auto block_sum64 = [&](u64 v) {
-        v = wave_sum64(v);
-        __syncthreads();
-        if (lane == 0) sh.wave64[wave] = v;
-        __syncthreads();
-        u64 t = 0;
-        for (int w = 0; w < WAVES; w++) t += sh.wave64[w];
-        __syncthreads();
-        return t;
+    // counts need 32 bits of a bin: half the LDS traffic
+    auto bin_at = [&](auto by_mass, int i) -> u64 { return decltype(by_mass)::value ? sh.hist[i] : (u64)((const unsigned*)sh.hist)[i]; };
+    auto add = [&](auto by_mass, int bin, float x) {
+        if constexpr (decltype(by_mass)::value) atomicAdd(&sh.hist[bin], Weight::integer(wt.scaled(x)));
+        else atomicAdd((unsigned*)sh.hist + bin, 1u);
     };
-    bool listed = false;               // sh.kept holds every kept id
-    // narrows (thr, thr_id) to the ids whose better ones measure less than the target.  The ids come from the row, or from sh.kept where that has them all.
-    auto select = [&](auto by_mass, u64 count) {
-        constexpr bool MASS = decltype(by_mass)::value;
+    auto clear = [&]() {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < BPT; i++) sh.hist[BPT * tid + i] = 0;
+        if (tid == 0) { sh.n_list = 0; sh.key_lo = 0xffffffffu; sh.key_hi = 0; sh.found = -1; }
+        __syncthreads();
+    };
+    auto my_bins = [&](auto by_mass) {
+        u64 s = 0;
+#pragma unroll
+        for (int i = 0; i < BPT; i++) s += bin_at(by_mass, BPT * tid + i);
+        return s;
+    };
+    // finds the crossing of `target` in hist (bins in order from the best): bin in sh.found, measure before it in sh.found_base
+    auto cross = [&](auto by_mass, u64 base, u64 target) {
+        const u64 own = my_bins(by_mass), inc = wave_scan64(own, lane);
+        if (lane == 63) sh.wave64[wave] = inc;
+        __syncthreads();
+        u64 before = base + inc - own;
+        for (int w = 0; w < wave; w++) before += sh.wave64[w];
+#pragma unroll
+        for (int i = 0; i < BPT; i++) {
+            const u64 h = bin_at(by_mass, BPT * tid + i);
+            if (before < target && target <= before + h) { sh.found = BPT * tid + i; sh.found_base = before; }
+            before += h;
+        }
+        __syncthreads();
+    };
+    const std::integral_constant<bool, false> by_count{};
+    const std::integral_constant<bool, true> by_mass{};
+
+    bool listed = false;               // sh.kept holds every id that is still kept (and others, that `alive` rules out)
+    // the ids of the histogram's steps 0 .. b - 1 into sh.kept, those of step b into sh.list with their measure.  Almost every id falls to one comparison
+    // with a bound below them all
+    auto list_steps = [&](auto mode, int b) {
+        const float reach = top - (float)(b + 2) / steps - fabsf(top) * 4e-7f - 1e-37f;      // (b + 1) / steps and what float32 may be off
+        __syncthreads();
+        if (tid == 0) { sh.n_kept = 0; sh.n_list = 0; sh.key_lo = 0xffffffffu; sh.key_hi = 0; }
+        __syncthreads();
+        unsigned key_lo = 0xffffffffu, key_hi = 0;
+        const bool sum = a.logprob && by_k && !summed;
+        over_row([&](int, int i0, const float* x) {
+            if (sum) add_parts(x);
+            float m = x[0];
+#pragma unroll
+            for (int e = 1; e < VEC; e++) m = fmaxf(m, x[e]);
+            if (!__ballot(m >= reach)) return;
+            const bool full = *(volatile int*)&sh.n_kept > kList;         // of no use any more
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                if (!(x[e] >= reach && x[e] > -kInf)) continue;
+                const int bin = bin_of(x[e]);
+                const unsigned key = order_key(x[e]);
+                if (bin == b) {
+                    const int at = atomicAdd(&sh.n_list, 1);
+                    if (at < kList) sh.list[at] = Entry{key, i0 + e, decltype(mode)::value ? Weight::integer(wt.scaled(x[e])) : 1};
+                    key_lo = min(key_lo, key);
+                    key_hi = max(key_hi, key);
+                } else if (bin < b && !full) {
+                    const int at = atomicAdd(&sh.n_kept, 1);
+                    if (at < kList) sh.kept[at] = Entry{key, i0 + e, 0};
+                }
+            }
+        });
+        if (key_lo <= key_hi) { atomicMin(&sh.key_lo, key_lo); atomicMax(&sh.key_hi, key_hi); }
+        if (sum) { sum_parts(); summed = true; }
+        __syncthreads();
+    };
+    // narrows (thr, thr_id) to the ids whose better ones measure less than the target, from sh.kept or from the row.  target 0: top_p of the measure's total.
+    // `complete`: the source holds every id that (thr, thr_id) keeps, so that there may be nothing to narrow.  b >= 0: the target is known to be crossed
+    // in step b, `base` lies before it
+    auto select = [&](auto mode, auto from_list, u64 target, bool complete, int b, u64 base) {
+        constexpr bool MASS = decltype(mode)::value, LIST = decltype(from_list)::value;
         auto measure = [&](float x) -> u64 { return MASS ? Weight::integer(wt.scaled(x)) : 1; };
-        const bool from_list = listed;
-        const int n_from = listed ? sh.n_kept : 0;
+        const int n_from = LIST ? sh.n_kept : 0;
         auto each = [&](auto f) {                                         // f(logit, id) of every id still kept
-            if (from_list) {
-                for (int i = tid; i < n_from; i += THREADS) f(value_of(sh.kept[i].key), sh.kept[i].id);
-            } else {
+            if constexpr (LIST) {
+                for (int i = tid; i < n_from; i += THREADS) {
+                    const float x = value_of(sh.kept[i].key);
+                    if (alive(x, sh.kept[i].id)) f(x, sh.kept[i].id);
+                }
+            } else
                 over_row([&](int, int i0, const float* x) {
 #pragma unroll
                     for (int e = 0; e < VEC; e++)
                         if (alive(x[e], i0 + e)) f(x[e], i0 + e);
                 });
-            }
-        };
-        // counts need 32 bits: half the LDS traffic
-        auto add = [&](int bin, float x) {
-            if constexpr (MASS) atomicAdd(&sh.hist[bin], measure(x));
-            else atomicAdd((unsigned*)sh.hist + bin, 1u);
-        };
-        auto bin_at = [&](int i) -> u64 { return MASS ? sh.hist[i] : (u64)((const unsigned*)sh.hist)[i]; };
-        auto my_bins = [&]() {
-            u64 s = 0;
-#pragma unroll
-            for (int i = 0; i < BPT; i++) s += bin_at(BPT * tid + i);
-            return s;
-        };
-        // finds the crossing of `target` in hist (bins in order from the best): bin in sh.found, measure before it in sh.found_base
-        auto cross = [&](u64 base, u64 target) {
-            const u64 mine = my_bins(), inc = wave_scan64(mine, lane);
-            if (lane == 63) sh.wave64[wave] = inc;
-            __syncthreads();
-            u64 before = base + inc - mine;
-            for (int w = 0; w < wave; w++) before += sh.wave64[w];
-#pragma unroll
-            for (int i = 0; i < BPT; i++) {
-                const u64 h = bin_at(BPT * tid + i);
-                if (before < target && target <= before + h) { sh.found = BPT * tid + i; sh.found_base = before; }
-                before += h;
-            }
-            __syncthreads();
-        };
-        auto clear = [&]() {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < BPT; i++) sh.hist[BPT * tid + i] = 0;
-            if (tid == 0) { sh.n_list = 0; sh.key_lo = 0xffffffffu; sh.key_hi = 0; sh.found = -1; }
-            __syncthreads();
         };
         auto take = [&](float x, int id) {                                // into the list of candidates
             const unsigned key = order_key(x);
@@ -312,41 +392,27 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
             atomicMin(&sh.key_lo, key);
             atomicMax(&sh.key_hi, key);
         };
-        clear();
-        if (!MASS && a.logprob) {      // the pass that counts also sums up what logprob needs
-            over_row([&](int, int i0, const float* x) {
-                add_parts(x);
-#pragma unroll
-                for (int e = 0; e < VEC; e++)
-                    if (x[e] > -kInf) add(bin_of(x[e]), x[e]);
-            });
-        } else each([&](float x, int) { add(bin_of(x), x); });
-        __syncthreads();
-        if (!MASS && a.logprob) sum_parts();
-        const u64 total = block_sum64(my_bins());
-        if (MASS && !by_k) whole = (double)total / one;
-        u64 target = count;
-        if constexpr (MASS) target = max((u64)1, (u64)ceil((double)fmaxf(p_row, 0.0f) * (double)total));
-        if (target >= total) return;                                      // all of them
-        cross(0, target);
-        int b = sh.found;
-        u64 base = sh.found_base;
-        if (from_list) each([&](float x, int id) { if (bin_of(x) == b) take(x, id); });
-        else {
-            if (tid == 0) sh.n_kept = 0;
+        if (b < 0) {
+            clear();
+            each([&](float x, int) { add(mode, bin_of(x), x); });
             __syncthreads();
-            each([&](float x, int id) {
-                const int y = bin_of(x);
-                if (y == b) take(x, id);
-                else if (y < b) {
-                    const int at = atomicAdd(&sh.n_kept, 1);
-                    if (at < kList) sh.kept[at] = Entry{order_key(x), id, 0};
-                }
-            });
+            const u64 total = block_sum64(my_bins(mode));
+            if (target == 0) target = max((u64)1, (u64)ceil((double)fmaxf(p_row, 0.0f) * (double)total));
+            if (target >= total && complete) return;
+            target = min(target, total);
+            cross(mode, 0, target);
+            b = sh.found; base = sh.found_base;
         }
-        __syncthreads();
-        const bool first = sh.n_list <= kList;                            // the candidates are all of one histogram step
-        for (;;) {
+        const bool fresh = thr == -kInf;                                  // nothing is ruled out yet: the row's steps are what is kept
+        if constexpr (LIST) {
+            each([&](float x, int id) { if (bin_of(x) == b) take(x, id); });
+            __syncthreads();
+        } else if (fresh) list_steps(mode, b);
+        else {
+            each([&](float x, int id) { if (bin_of(x) == b) take(x, id); });
+            __syncthreads();
+        }
+        for (bool first = true;; first = false) {
             const int n = sh.n_list;
             const unsigned lo = sh.key_lo, hi = sh.key_hi;
             __syncthreads();
@@ -360,7 +426,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
                 }
                 __syncthreads();
                 thr = value_of(sh.found_key); thr_id = sh.found_id;
-                if (!from_list && first) {
+                if (!LIST && fresh && first) {                            // the candidates that stay join the better steps
                     for (int i = tid; i < n; i += THREADS)
                         if (alive(value_of(sh.list[i].key), sh.list[i].id)) {
                             const int at = atomicAdd(&sh.n_kept, 1);
@@ -374,31 +440,9 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
             if (lo == hi) {                                               // equal logits: the first `need` of them by id
                 const float tie = value_of(lo);
                 const u64 m = measure(tie), need = (target - base + m - 1) / m;
-                auto ties = [&](int i0, const float* x) {                 // this lane's ties of a group
-                    int n = 0;
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) n += x[e] == tie && alive(tie, i0 + e);
-                    return n;
-                };
-                over_row([&](int g, int i0, const float* x) {
-                    const u64 n = wave_sum64((u64)ties(i0, x));
-                    if (lane == 0) mass[g] = n;
-                });
-                __syncthreads();
-                if (wave == 0) {
-                    u64 run = 0;
-                    int at = 0;
-                    for (; at < r.groups - 1 && run + mass[at] < need; at++) run += mass[at];
-                    float x[VEC];
-                    const int i0 = r.load(at, lane, x);
-                    const u64 mine = (u64)ties(i0, x), inc = run + wave_scan64(mine, lane);
-                    if (inc - mine < need && need <= inc) {
-                        u64 n = inc - mine;
-#pragma unroll
-                        for (int e = 0; e < VEC; e++)
-                            if (x[e] == tie && alive(tie, i0 + e) && ++n == need) sh.found_id = i0 + e;
-                    }
-                }
+                auto is = [&](float x, int id) { return x == tie && alive(tie, id); };
+                count_groups(is);
+                if (wave == 0) nth(need, is);
                 __syncthreads();
                 thr = tie; thr_id = sh.found_id;
                 return;
@@ -407,10 +451,10 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
             clear();
             each([&](float x, int) {
                 const unsigned key = order_key(x);
-                if (key >= lo && key <= hi) add((int)((hi - key) >> shift), x);
+                if (key >= lo && key <= hi) add(mode, (int)((hi - key) >> shift), x);
             });
             __syncthreads();
-            cross(base, target);
+            cross(mode, base, target);
             b = sh.found; base = sh.found_base;
             each([&](float x, int id) {
                 const unsigned key = order_key(x);
@@ -419,8 +463,43 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
             __syncthreads();
         }
     };
-    if (by_k) select(std::integral_constant<bool, false>(), (u64)k_row);
-    if (by_p) select(std::integral_constant<bool, true>(), 0);
+    const std::integral_constant<bool, true> from_list{};
+    const std::integral_constant<bool, false> from_row{};
+    if (by_k) {
+        // the k-th largest of the threads' largest logits bounds the k-th largest of all from below.  For k of half the threads about 0.7 THREADS ids of a
+        // random row lie above it: the list takes them, and they are all that is looked at from here on
+        if (2 * k_row <= THREADS) {
+            clear();
+            if (mine > -kInf) add(by_count, bin_of(mine), mine);
+            __syncthreads();
+            if (block_sum64(my_bins(by_count)) >= (u64)k_row) {
+                cross(by_count, 0, (u64)k_row);
+                list_steps(by_count, sh.found + 1);
+                listed = sh.n_kept <= kList;
+            }
+        }
+        if (listed) select(by_count, from_list, (u64)k_row, false, -1, 0);
+        else select(by_count, from_row, (u64)k_row, true, -1, 0);
+    }
+    if (by_p) {
+        if (listed) select(by_mass, from_list, 0, true, -1, 0);
+        else if (by_k) select(by_mass, from_row, 0, true, -1, 0);
+        else {
+            // masked ids and NaN weigh 0: no test
+            clear();
+            over_row([&](int, int, const float* x) {
+#pragma unroll
+                for (int e = 0; e < VEC; e++) add(by_mass, bin_of(x[e]), x[e]);
+            });
+            __syncthreads();
+            const u64 total = block_sum64(my_bins(by_mass)), target = max((u64)1, (u64)ceil((double)fmaxf(p_row, 0.0f) * (double)total));
+            whole = (double)total / one;
+            if (target < total) {
+                cross(by_mass, 0, target);
+                select(by_mass, from_row, target, true, sh.found, sh.found_base);
+            }
+        }
+    }
 
     // the kept ids' weights, group by group
     auto kept = [&](float x, int id, u64* w) {
@@ -441,14 +520,19 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
             if (kept(value_of(e.key), e.id, &w)) { total += w; n_kept++; atomicAdd(&mass[e.id / R::GROUP], w); }
         }
     } else {
-        const bool add_whole = a.logprob && by_m && !by_k && !by_p;
+        const bool add_whole = a.logprob && !summed && (by_k || (by_m && !by_p)), plain_row = !by_k && !by_p && !by_m;
         over_row([&](int g, int i0, const float* x) {
             u64 s = 0;
             if (add_whole) add_parts(x);
+            if (plain_row) {                                              // masked ids and NaN weigh 0
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                u64 w;
-                if (kept(x[e], i0 + e, &w)) { s += w; n_kept++; }
+                for (int e = 0; e < VEC; e++) { s += Weight::integer(wt.scaled(x[e])); n_kept += x[e] > -kInf; }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    u64 w;
+                    if (kept(x[e], i0 + e, &w)) { s += w; n_kept++; }
+                }
             }
             total += s;
             s = wave_sum64(s);
