@@ -126,7 +126,8 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
 
     // f(group, first id of the lane, its VEC logits) over the wave's groups, the loads of the next AHEAD groups in flight.  f appears once in a rolled
     // loop: a workgroup runs through its code only a few times, and instruction fetches cost more than the moves between the buffers.
-    auto over_row = [&](auto f) {
+    // (inlined by force, as the passes below: a call keeps this kernel's variables in memory, 61 against 42 us for a row)
+    auto over_row = [&](auto f) __attribute__((always_inline)) {
         typename R::V v[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) v[i] = r.fetch(wave + i * WAVES, lane);
@@ -197,7 +198,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
                 if (is(x[e], i0 + e) && ++n == need) sh.found_id = i0 + e;
         }
     };
-    auto count_groups = [&](auto is) {
+    auto count_groups = [&](auto is) __attribute__((always_inline)) {
         over_row([&](int g, int i0, const float* x) {
             u64 n = 0;
 #pragma unroll
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
     bool listed = false;               // sh.kept holds every id that is still kept (and others, that `alive` rules out)
     // the ids of the histogram's steps 0 .. b - 1 into sh.kept, those of step b into sh.list with their measure.  Almost every id falls to one comparison
     // with a bound below them all
-    auto list_steps = [&](auto mode, int b) {
+    auto list_steps = [&](auto mode, int b) __attribute__((always_inline)) {
         const float reach = top - (float)(b + 2) / steps - fabsf(top) * 4e-7f - 1e-37f;      // (b + 1) / steps and what float32 may be off
         __syncthreads();
         if (tid == 0) { sh.n_kept = 0; sh.n_list = 0; sh.key_lo = 0xffffffffu; sh.key_hi = 0; }
@@ -368,11 +369,11 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
     // narrows (thr, thr_id) to the ids whose better ones measure less than the target, from sh.kept or from the row.  target 0: top_p of the measure's total.
     // `complete`: the source holds every id that (thr, thr_id) keeps, so that there may be nothing to narrow.  b >= 0: the target is known to be crossed
     // in step b, `base` lies before it
-    auto select = [&](auto mode, auto from_list, u64 target, bool complete, int b, u64 base) {
+    auto select = [&](auto mode, auto from_list, u64 target, bool complete, int b, u64 base) __attribute__((always_inline)) {
         constexpr bool MASS = decltype(mode)::value, LIST = decltype(from_list)::value;
         auto measure = [&](float x) -> u64 { return MASS ? Weight::integer(wt.scaled(x)) : 1; };
         const int n_from = LIST ? sh.n_kept : 0;
-        auto each = [&](auto f) {                                         // f(logit, id) of every id still kept
+        auto each = [&](auto f) __attribute__((always_inline)) {                                         // f(logit, id) of every id still kept
             if constexpr (LIST) {
                 for (int i = tid; i < n_from; i += THREADS) {
                     const float x = value_of(sh.kept[i].key);
@@ -404,10 +405,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
             b = sh.found; base = sh.found_base;
         }
         const bool fresh = thr == -kInf;                                  // nothing is ruled out yet: the row's steps are what is kept
-        if constexpr (LIST) {
-            each([&](float x, int id) { if (bin_of(x) == b) take(x, id); });
-            __syncthreads();
-        } else if (fresh) list_steps(mode, b);
+        if (!LIST && fresh) list_steps(mode, b);
         else {
             each([&](float x, int id) { if (bin_of(x) == b) take(x, id); });
             __syncthreads();
@@ -437,6 +435,7 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
                 }
                 return;
             }
+            if constexpr (LIST) return;                                   // never: a list's ids fit
             if (lo == hi) {                                               // equal logits: the first `need` of them by id
                 const float tie = value_of(lo);
                 const u64 m = measure(tie), need = (target - base + m - 1) / m;
@@ -448,18 +447,20 @@ __global__ __launch_bounds__(THREADS) void sample_rows_kernel(ss_sample_rows_arg
                 return;
             }
             const int shift = max(0, 32 - __clz(hi - lo) - 11);
+            auto in_reach = [&](auto f) {                                 // f(logit, id, key) of the kept ids with keys from lo to hi.  One id at a time: rare
+#pragma unroll 1
+                for (int i = tid; i < r.n; i += THREADS) {
+                    const float x = (float)r.p[i];
+                    const unsigned key = order_key(x);
+                    if (key >= lo && key <= hi && alive(x, i)) f(x, i, key);
+                }
+            };
             clear();
-            each([&](float x, int) {
-                const unsigned key = order_key(x);
-                if (key >= lo && key <= hi) add(mode, (int)((hi - key) >> shift), x);
-            });
+            in_reach([&](float x, int, unsigned key) { add(mode, (int)((hi - key) >> shift), x); });
             __syncthreads();
             cross(mode, base, target);
             b = sh.found; base = sh.found_base;
-            each([&](float x, int id) {
-                const unsigned key = order_key(x);
-                if (key >= lo && key <= hi && (int)((hi - key) >> shift) == b) take(x, id);
-            });
+            in_reach([&](float x, int id, unsigned key) { if ((int)((hi - key) >> shift) == b) take(x, id); });
             __syncthreads();
         }
     };
