@@ -6,6 +6,7 @@ can be captured into a graph.  Wrong arguments raise ValueError (or SpeakSenseEr
 from __future__ import annotations
 
 import ctypes as C
+from numbers import Integral
 from typing import NamedTuple
 
 import torch      # before the library: both must share one HIP runtime, torch's, and the loader keeps the first
@@ -142,7 +143,8 @@ class KvBatch:
         n, pages = page_table.shape
         _need(kv_len.numel() == n and q_start.numel() == n + 1, f"{n} rows of page_table, {kv_len.numel()} lengths, {q_start.numel()} starts")
         _need((pages <= 1 or page_table.stride(1) == 1) and (n == 0 or (kv_len.is_contiguous() and q_start.is_contiguous())), "rows of page_table, q_start and kv_len must be contiguous")
-        _need(all(isinstance(x, int) and 0 <= x < 1 << 31 for x in (n_tokens, max_new, min_new, max_len)), "n_tokens, max_new, min_new and max_len must be host integers in [0, 2^31)")
+        _need(all(isinstance(x, Integral) and 0 <= x < 1 << 31 for x in (n_tokens, max_new, min_new, max_len)), "n_tokens, max_new, min_new and max_len must be host integers in [0, 2^31)")
+        n_tokens, max_new, min_new, max_len = int(n_tokens), int(max_new), int(min_new), int(max_len)      # numpy's too
         self.page_table, self.q_start, self.kv_len, self.device, self.index = page_table, q_start, kv_len, page_table.device, page_table.get_device()
         self.n_seqs, self.n_tokens, self.max_new = n, n_tokens, max_new
         stride = page_table.stride(0) if n > 1 else pages
