@@ -393,9 +393,9 @@ typedef struct ss_kv_batch {      /* the sequences of one step */
     int64_t table_stride;         /* elements between rows of page_table, >= max_pages */
     int32_t n_seqs;
     int32_t max_pages;            /* max_pages * page_size < 2^30 */
-    int32_t n_tokens;             /* rows of the token tensors */
+    int32_t n_tokens;             /* rows of the token tensors, <= 2^24 */
     int32_t max_new;              /* at least the longest span (what a scheduler knows on the host): ss_kv_attention covers max_new tokens per sequence */
-    int32_t min_new;              /* the shortest span, or 0 if unknown: a hint that can save a launch */
+    int32_t min_new;              /* the shortest span, or 0 if unknown: a hint, of no effect where the kernels take any mixture as fast (as they do) */
     int32_t max_len;              /* about the longest kv_len, or 0 if unknown: decides only how the keys are cut over workgroups */
 } ss_kv_batch;
 typedef struct ss_kv_rows {       /* [n_tokens][heads][head_dim] of dtype: 16-byte aligned, the head's elements contiguous */
@@ -419,20 +419,20 @@ int ss_kv_read(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_r
  * and values that some token of the sequence sees are taken to be finite.
  * out: as q.  lse (optional): float32 [n_tokens][n_heads], the natural logarithm of the softmax's denominator, with which results over disjoint keys
  * are joined.  Softmax and sums are held in float32; the probabilities are rounded to the type that the matrix product takes (dtype; f16 for 8-bit
- * caches, whose codes it holds exactly).  Results do not depend on the run, but the order of their sums does on max_new, min_new, max_len and n_seqs.
+ * caches, whose codes it holds exactly).  Results do not depend on the run, but the order of their sums does on max_new, max_len and n_seqs.
  * workspace: ss_kv_attention_workspace(...) bytes, 16-byte aligned, NULL if that is 0; contents before and after mean nothing. */
 int64_t ss_kv_attention_workspace(const ss_kv_cache* cache, const ss_kv_batch* batch, int32_t n_heads);   /* < 0: SS_ERR_ARG.  Host only */
 int ss_kv_attention(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_rows* q, int32_t n_heads, float scale, int32_t causal, const ss_kv_rows* out,
                     float* lse, void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
 
 /* Draws one id per row of logits.  With x the row (NaN counts as -inf, "masked") and t its temperature, w_i = exp((x_i - max x) / t); ids at +inf share all
- * weight.  The filters, in this order: top_k keeps the k largest logits (ties: the lowest ids); top_p keeps an id while those before it, in order of
+ * weight, the others then count as masked.  The filters, in this order: top_k keeps the k largest logits (ties: the lowest ids); top_p keeps an id while those before it, in order of
  * weight (ties: of id), have less than top_p of what top_k left; min_p keeps ids with w_i >= min_p.  The best id is always kept.  Drawn is the first kept id, in
  * order of id, whose running sum of kept weights exceeds u times their total: std::discrete_distribution's rule for a given uniform number.
- * Weights are held as integers of 2^-bits of the largest (bits = 62 - log2 of the vocabulary, rounded down), so sums are exact and
+ * Weights are held as integers of 2^-bits of the largest (bits = 62 - log2 of the vocabulary, rounded down, 51 at most), so sums are exact and
  * do not depend on the order; a draw can differ from the real numbers' only where u falls within about 1e-12 of a boundary.
  * Settings per row may be NULL (off; temperature 1) and need no host value: t <= 0 or NaN takes the best id, top_k <= 0 or >= n_vocab, top_p >= 1 or NaN, min_p <= 0
- * or NaN switch a filter off; u is taken into [0, 1).  A row without any unmasked id gives id -1, p 0, logprob -inf, n_kept 0. */
+ * or NaN switch a filter off; min_p > 1 counts as 1; u is taken into [0, 1).  A row without any unmasked id gives id -1, p 0, logprob -inf, n_kept 0. */
 typedef struct ss_sample_rows_args {
     const void* logits;           /* [n_rows] rows of n_vocab, dtype, aligned to its size */
     const double* u;              /* [n_rows] uniform numbers; the engine's generator gives doubles too */
@@ -445,7 +445,7 @@ typedef struct ss_sample_rows_args {
     float* logprob;               /* ln of its probability before the filters, at temperature t (1 where t <= 0); may be NULL */
     int32_t* n_kept;              /* ids left by the filters (1 where t <= 0); may be NULL */
     int64_t row_stride;           /* elements, >= n_vocab */
-    int32_t n_rows;
+    int32_t n_rows;               /* <= 2^21 */
     int32_t n_vocab;              /* <= 2^20 */
     int32_t dtype;                /* SS_DTYPE_F32, SS_DTYPE_F16 or SS_DTYPE_BF16 */
     int32_t reserved;

@@ -567,7 +567,7 @@ const char* bad_cache(const ss_kv_cache& c) {
 }
 const char* bad_batch(const ss_kv_batch& b, const ss_kv_cache& c) {
     if (b.n_seqs < 0 || b.n_tokens < 0 || b.max_new < 0 || b.min_new < 0 || b.max_len < 0) return "negative size";
-    if (b.n_seqs > 1 << 20 || b.n_tokens > 1 << 28) return "too many sequences or tokens";
+    if (b.n_seqs > 1 << 20 || b.n_tokens > 1 << 24) return "too many sequences or tokens";
     if (b.max_pages <= 0 || (int64_t)b.max_pages * c.page_size >= (int64_t)1 << 30) return "max_pages * page_size must lie in (0, 2^30)";
     if (b.table_stride < b.max_pages) return "table_stride is smaller than max_pages";
     if (b.n_seqs > 0 && (!b.page_table || !b.q_start || !b.kv_len)) return "null page_table, q_start or kv_len";
@@ -668,7 +668,7 @@ int ss_sample_rows(const ss_sample_rows_args* a, int32_t device, void* stream) {
     const int size = a->dtype == SS_DTYPE_F32 ? 4 : 2;
     const char* why = nullptr;
     if (a->dtype != SS_DTYPE_F32 && a->dtype != SS_DTYPE_F16 && a->dtype != SS_DTYPE_BF16) why = "dtype must be SS_DTYPE_F32, SS_DTYPE_F16 or SS_DTYPE_BF16";
-    else if (a->n_rows < 0 || a->n_rows > 1 << 24) why = "n_rows must lie in [0, 2^24]";
+    else if (a->n_rows < 0 || a->n_rows > 1 << 21) why = "n_rows must lie in [0, 2^21]";
     else if (a->n_vocab <= 0 || a->n_vocab > 1 << 20) why = "n_vocab must lie in [1, 2^20]";
     else if (a->row_stride < a->n_vocab || a->row_stride > (int64_t)1 << 40) why = "row_stride is smaller than n_vocab";
     else if (a->n_rows > 0 && (!a->logits || !a->u || !a->id)) why = "null logits, u or id";

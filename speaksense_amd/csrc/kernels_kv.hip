@@ -267,7 +267,7 @@ struct AttnArgs {
     float c2;                          // |scale| * log2(e), at least the smallest normal number: a masked -inf stays one
     int neg;                           // scale < 0: the queries' signs are turned instead
     int G, causal, splits, split_keys; // query heads per key head; key ranges and their length (a multiple of 128)
-    int all, nq;                       // tile kernel: also the sequences of at most 16 query rows; query tiles per (sequence, head)
+    int nq;                            // tile kernel: query tiles per (sequence, head)
 };
 
 constexpr float kInf = __builtin_huge_valf();
@@ -481,7 +481,7 @@ template <typename T, int N> __device__ __forceinline__ void store_cols(T* p, co
     }
 }
 
-// ---- few query rows (n_new G <= 16): grid (sequences x splits, key heads); the 4 waves of a workgroup take every fourth 32-key tile of its key
+// ---- few query rows (n_new G <= 16 in every sequence): grid (sequences x splits, key heads); the 4 waves of a workgroup take every fourth 32-key tile of its key
 // range straight from memory into registers (the next tile's loads fly while one is computed) and merge at the end.  HBM-bound: with G <= 16 the
 // MFMA issues of a tile take ~1/10 of the time its bytes need at the card's rate, so the 15 idle columns of a one-head row cost nothing. ----
 template <int KIND, int D> struct KvTile {
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     const int h = bid % a.H, s = bid / a.H;
     const Span sp = seq_span(a, s);
     const int rows = sp.n_new * t.G, r0 = qb * (64 * QC);
-    if (rows <= r0 || (rows <= 16 && !t.all)) return;
+    if (rows <= r0) return;
 
     const int w0 = r0 + wave * (16 * QC);                  // this wave's first query row
     int limit[QC];
@@ -958,10 +958,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     }
 }
 
-// One workgroup per query row joins its key ranges: 4 waves take them in turn, 8 loads in flight each.  `few`: rows of the few-row kernel (n_new G <= 16),
-// else those of the tile kernel (`all`: every row).
+// One workgroup per query row joins its key ranges: 4 waves take them in turn, 8 loads in flight each.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t, int few) {
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t) {
     constexpr int E = D / 64;
     __shared__ float s_acc[4][D];
     const int heads = a.H * t.G, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -971,7 +970,6 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t,
     if (s < 0 || s >= a.n_seqs) return;
     const Span sp = seq_span(a, s);
     if (row < sp.q0 || row >= sp.q0 + sp.n_new) return;
-    if (!t.all && (sp.n_new * t.G <= 16) != (few != 0)) return;
     const float2 ml = lane < t.splits ? t.part_ml[at * t.splits + lane] : make_float2(-kInf, 0.0f);
     const float m = wave_max(ml.x), f = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
     const float L = wave_sum(ml.y * f);
@@ -1064,29 +1062,29 @@ void launch_kv_read(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows
     SS_LAUNCH_CHECK();
 }
 
-// Up to so many keys a batch that mixes chunks with short spans runs on the tile kernel alone
-constexpr long kTileTakesAll = 2048;
-
 KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads) {
     KvPlan p{};
-    p.few_splits = p.tile_splits = 1;
+    p.splits = 1;
     if (b.n_seqs == 0 || b.n_tokens == 0 || b.max_new == 0) return p;
+    const bool join = (long)b.n_tokens * n_heads < 1 << 24;        // a workgroup a row: more than that is no grid, and fills the card without cuts
     const int G = n_heads / c.n_kv_heads;
     const long cap = (long)b.max_pages * c.page_size, keys = std::max(1l, b.max_len > 0 ? std::min((long)b.max_len, cap) : cap);
     const long rows = (long)b.max_new * G, pairs = (long)b.n_seqs * c.n_kv_heads;
+    // One kernel takes the whole batch: a workgroup of the tile kernel that finds few rows leaves three waves to the loads alone.  The few-row kernel beside it for
+    // the spans of up to 16 rows, with a join of its own, was slower wherever both apply: 32 spans of 1..20 rows over 448 keys 27 us against 17, over 16384 keys
+    // 689 against 460
     p.tile = rows > 16;
-    p.few = !p.tile || ((long)std::max(b.min_new, 1) * G <= 16 && keys > kTileTakesAll);
-    p.qc = rows <= 64 ? 1 : rows < 1024 || c.head_dim == 128 ? 2 : 4;
-    p.few_keys = p.tile_keys = (int)std::min(keys, 1l << 30);
-    auto cut = [&](long groups, long want, int least, int* splits, int* len) {   // as many key ranges as fill the card, none shorter than `least`
-        const long n = std::max(1l, std::min({(want + groups - 1) / groups, (keys + least - 1) / least, 64l}));
-        *len = (int)((keys + n * 128 - 1) / (n * 128) * 128);
-        *splits = (int)((keys + *len - 1) / *len);
-    };
-    if (p.few) cut(pairs, 512, 512, &p.few_splits, &p.few_keys);
-    if (p.tile) cut(pairs * up(rows, 64 * p.qc), 512, 512, &p.tile_splits, &p.tile_keys);
-    const int n = std::max(p.few_splits, p.tile_splits);
-    if (n > 1) p.workspace = (int64_t)b.n_tokens * n_heads * n * (c.head_dim + 2) * 4;
+    // Column tiles a wave.  4 read K and V out of LDS half as often, if they leave two workgroups a CU (head_dim 64, int8: 8 x 512 x 4 rows 208 us against 256,
+    // but 8 x 256 x 4 rows, one workgroup a CU, 176 against 134); at head_dim 128 they do not fit the registers
+    const long wide = pairs * up(rows, 256);
+    p.qc = rows <= 64 ? 1 : c.head_dim == 64 && rows >= 1024 && wide >= 512 ? 4 : 2;
+    // As many key ranges as give the card 512 workgroups, none shorter than 512 keys (256 wanted: 1 x 128 x 4 rows over 16384 keys 87 us instead of 72; 1024 wanted:
+    // 83, and 16 contexts of one token 546 instead of 504)
+    const long groups = p.tile ? pairs * up(rows, 64 * p.qc) : pairs;
+    const long n = !join ? 1 : std::max(1l, std::min({(512 + groups - 1) / groups, (keys + 511) / 512, 64l}));
+    p.split_keys = (int)((keys + n * 128 - 1) / (n * 128) * 128);
+    p.splits = (int)((keys + p.split_keys - 1) / p.split_keys);
+    if (p.splits > 1) p.workspace = (int64_t)b.n_tokens * n_heads * p.splits * (c.head_dim + 2) * 4;
     return p;
 }
 
@@ -1099,40 +1097,30 @@ void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv
     t.q = q.p; t.q_row = q.row_stride; t.q_head = q.head_stride;
     t.out = out.p; t.o_row = out.row_stride; t.o_head = out.head_stride;
     t.lse = lse; t.c2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f); t.neg = scale < 0.0f; t.G = n_heads / c.n_kv_heads; t.causal = causal;
-    t.all = p.tile && !p.few;
     by_type(c, [&](auto tt, auto kind, auto dim) {
         typedef decltype(tt) T;
         constexpr int K = kind.value, D = dim.value;
-        auto join = [&](int few) {
-            if (t.splits == 1) return;
-            kv_attn_join_kernel<T, D><<<(unsigned)((long)b.n_tokens * n_heads), 256, 0, st>>>(a, t, few);
-            SS_LAUNCH_CHECK();
-        };
-        auto part = [&](int splits, int keys) {            // the two kernels follow each other on the stream: they may share the workspace
-            t.splits = splits; t.split_keys = keys;
-            t.part = (float*)workspace;
-            t.part_ml = (float2*)((float*)workspace + (size_t)b.n_tokens * n_heads * splits * D);
-        };
-        if (p.few) {
-            part(p.few_splits, p.few_keys);
-            kv_attn_few_kernel<T, K, D><<<dim3(b.n_seqs * p.few_splits, c.n_kv_heads), 256, 0, st>>>(a, t);
-            SS_LAUNCH_CHECK();
-            join(1);
-        }
-        if (p.tile) {
-            part(p.tile_splits, p.tile_keys);
+        t.splits = p.splits; t.split_keys = p.split_keys;
+        t.part = (float*)workspace;
+        t.part_ml = (float2*)((float*)workspace + (size_t)b.n_tokens * n_heads * p.splits * D);
+        if (!p.tile)
+            kv_attn_few_kernel<T, K, D><<<dim3(b.n_seqs * p.splits, c.n_kv_heads), 256, 0, st>>>(a, t);
+        else {
             auto go = [&](auto qc) {
                 constexpr int QC = qc.value, smem = 2 * kTileBuf<D>;
                 static std::atomic<uint64_t> once{0};
                 once_per_device(once, [&] { SS_HIP(hipFuncSetAttribute((const void*)kv_attn_tile_kernel<T, K, D, QC>, hipFuncAttributeMaxDynamicSharedMemorySize, smem)); });
                 t.nq = up((long)b.max_new * t.G, 64 * QC);
-                kv_attn_tile_kernel<T, K, D, QC><<<(unsigned)((long)b.n_seqs * c.n_kv_heads * t.nq * p.tile_splits), 256, smem, st>>>(a, t);
-                SS_LAUNCH_CHECK();
+                kv_attn_tile_kernel<T, K, D, QC><<<(unsigned)((long)b.n_seqs * c.n_kv_heads * t.nq * p.splits), 256, smem, st>>>(a, t);
             };
             if (p.qc == 1) go(Int<1>());
             else if (p.qc == 2 || D == 128) go(Int<2>());
             else if constexpr (D == 64) go(Int<4>());
-            join(0);
+        }
+        SS_LAUNCH_CHECK();
+        if (p.splits > 1) {
+            kv_attn_join_kernel<T, D><<<(unsigned)((long)b.n_tokens * n_heads), 256, 0, st>>>(a, t);
+            SS_LAUNCH_CHECK();
         }
     });
 }

@@ -11,10 +11,9 @@ void launch_kv_read(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv_rows
 
 // How one attention call is cut: a pure function of the host-known sizes, so that the workspace query and the launch agree.
 struct KvPlan {
-    bool few, tile;            // which kernels run: sequences of at most 16 query rows per key head / all others
+    bool tile;                 // the tile kernel; else that of at most 16 query rows per key head
     int qc;                    // tile kernel: 16-row column tiles per wave
-    int few_splits, few_keys;  // key ranges per sequence and their length
-    int tile_splits, tile_keys;
+    int splits, split_keys;    // key ranges per sequence and their length
     int64_t workspace;         // bytes of partial results
 };
 KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads);

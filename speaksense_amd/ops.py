@@ -97,7 +97,7 @@ class KvCache:
         _need(k.dtype in held and v.dtype == k.dtype, f"k and v must be {held[0]}, got {k.dtype} and {v.dtype}")
         _need(k.dim() == 4 and v.shape == k.shape, "k and v must be [n_pages, n_kv_heads, page_size, head_dim], alike")
         n, heads, page, dim = k.shape
-        _need(all(t.stride()[1:] == (page * dim, dim, 1) for t in (k, v)) and k.stride(0) == v.stride(0), "each page must be contiguous, k and v with one stride between pages")
+        _need(all(t.stride()[1:] == (page * dim, dim, 1) for t in (k, v)) and (n == 1 or k.stride(0) == v.stride(0)), "each page must be contiguous, k and v with one stride between pages")
         scales = None
         if self.kind == KV_SAME:
             _need(k_scale is None and v_scale is None, "a 16-bit cache has no scales")
@@ -106,12 +106,12 @@ class KvCache:
             for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
                 _on(t, k.device, name)
                 _need(t.dtype == scales and t.shape == k.shape[:3], f"{name} must be {scales} [n_pages, n_kv_heads, page_size]")
-                _need(t.stride()[1:] == (page, 1) and t.stride(0) == k_scale.stride(0), "each page's scales must be contiguous, with one stride between pages")
+                _need(t.stride()[1:] == (page, 1) and (n == 1 or t.stride(0) == k_scale.stride(0)), "each page's scales must be contiguous, with one stride between pages")
         self.k, self.v, self.k_scale, self.v_scale, self.dtype, self.device, self.index = k, v, k_scale, v_scale, dtype, k.device, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, heads, page, dim
         # a cache of one page may be a view whose stride says nothing
-        page_stride = k.stride(0) if n > 1 else max(k.stride(0), heads * page * dim)
-        scale_stride = 0 if scales is None else k_scale.stride(0) if n > 1 else max(k_scale.stride(0), heads * page)
+        page_stride = k.stride(0) if n > 1 else heads * page * dim
+        scale_stride = 0 if scales is None else k_scale.stride(0) if n > 1 else heads * page
         self._c = _Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if scales is not None else None, v_scale.data_ptr() if scales is not None else None,
                          page_stride, scale_stride, n, page, heads, dim, _DTYPES[dtype], self.kind)
 
