@@ -339,7 +339,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     // the ids of the histogram's steps 0 .. b - 1 into sh.kept, those of step b into sh.list with their measure.  Almost every id falls to one comparison
     // with a bound below them all
     auto list_steps = [&](auto mode, int b) __attribute__((always_inline)) {
-        const float reach = top - (float)(b + 2) / steps - fabsf(top) * 4e-7f - 1e-37f;      // (b + 1) / steps and what float32 may be off
+        // (b + 1) / steps and what float32 may be off; the last step holds all that lies below it too
+        const float reach = b >= kBins - 1 ? -kInf : top - (float)(b + 2) / steps - fabsf(top) * 4e-7f - 1e-37f;
         __syncthreads();
         if (tid == 0) { sh.n_kept = 0; sh.n_list = 0; sh.key_lo = 0xffffffffu; sh.key_hi = 0; }
         __syncthreads();

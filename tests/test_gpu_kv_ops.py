@@ -615,3 +615,21 @@ def test_the_current_device_stays():
     assert torch.cuda.current_device() == 0
     assert L.ss_kv_append(c._c, b._c, r, r, 0, None) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_cache_of_one_page(kind):
+    """The stride over a single page says nothing: a slice of a pool with any stride is taken."""
+    held = {"same": torch.float16, "e4m3": torch.uint8, "int8": torch.int8}[kind]
+    pool = torch.zeros(2 * 2 * 16 * 64, dtype=held, device="cuda")
+    k, v = (torch.as_strided(pool, (1, 2, 16, 64), (stride, 1024, 64, 1), at) for stride, at in ((7, 0), (1 << 33, 2048)))
+    scales = [] if kind == "same" else [torch.as_strided(torch.zeros(32, dtype=torch.uint8 if kind == "e4m3" else torch.float32, device="cuda"), (1, 2, 16), (s, 16, 1)) for s in (3, 5)]
+    c = ops.KvCache(k, v, *scales, kind=kind, dtype=torch.float16)
+    t32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    b = ops.KvBatch(t32(0)[None], t32(0, 5), t32(5), n_tokens=5, max_new=5)
+    x = torch.ones((5, 2, 64), dtype=torch.float16, device="cuda")
+    ops.kv_append(c, b, x, 2 * x)
+    rk, rv = ops.kv_read(c, b)
+    tol = 0 if kind != "int8" else 2.0 ** -11                            # 127 * (1 / 127 in float32) rounded to f16
+    assert float((rk - x).abs().max()) <= tol and float((rv - 2 * x).abs().max()) <= 2 * tol
+    assert float((ops.kv_attention(c, b, x) - 2.0).abs().max()) <= 2 * 2.0 ** -9

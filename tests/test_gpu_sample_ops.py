@@ -239,3 +239,26 @@ def test_captured_sampling():
         torch.cuda.synchronize()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(r, want)), i
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("share", [0.02, 0.995])
+def test_masks_of_the_lowest_number(dt, share):
+    """Ids that a mask holds at the type's lowest number are ordinary logits that weigh nothing; they must not blunt the histograms of the others."""
+    g = torch.Generator().manual_seed(12)
+    n, v = 8, 5000
+    x = (torch.randn((n, v), generator=g) * 3).to(dt)
+    x.masked_fill_(torch.rand((n, v), generator=g) < share, torch.finfo(dt).min)
+    x[-1].fill_(torch.finfo(dt).min)
+    u = torch.rand((n,), generator=g, dtype=torch.float64).tolist()
+    check(x, u, t=[0.7] * n, k=[0, 40, 900, 0, 7, 0, 1, 3], p=[1.0, 1.0, 1.0, 0.9, 0.8, 0.6, 1.0, 1.0], m=[0.0] * 4 + [0.02] * 4)
+
+
+def test_long_lists_and_wide_nuclei():
+    """top-k on both sides of the bound of 512, with more ids than the list of 1024 above the bound or in the nucleus, and logits of a wide span."""
+    g = torch.Generator().manual_seed(13)
+    for scale in (2.5, 40.0):
+        x = torch.randn((8, 30000), generator=g) * scale
+        x[6, 100:2000] = x[6].max()                                     # more best ids than the list holds
+        u = torch.rand((8,), generator=g, dtype=torch.float64).tolist()
+        check(x, u, t=[1.0, 1.0, 3.0, 2.0, 1.0, 4.0, 1.0, 2.0], k=[511, 512, 513, 1500, 20000, 0, 700, 0], p=[1.0, 0.9, 1.0, 0.99, 1.0, 0.97, 0.5, 0.9])

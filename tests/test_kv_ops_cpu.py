@@ -152,3 +152,16 @@ def test_host_tensors_are_refused():
         ops.KvBatch(torch.zeros(1, 2, dtype=torch.int32), i, i[:1], n_tokens=1, max_new=1)
     with pytest.raises(ValueError, match="device memory"):
         ops.sample_rows(torch.zeros(2, 10), torch.zeros(2, dtype=torch.float64))
+
+
+def test_sizes_that_are_no_grid_are_refused():
+    """A launch holds less than 2^32 threads: one workgroup of 256 per token row at most, one of 1024 per row of logits."""
+    for rc in _calls(_cache(), _batch(n_tokens=(1 << 24) + 1)):
+        _refused(rc, "too many")
+    d = dict(logits=P, u=P, temperature=None, top_k=None, top_p=None, min_p=None, id=P, p=None, logprob=None, n_kept=None, row_stride=100, n_rows=(1 << 21) + 1, n_vocab=100, dtype=3, reserved=0)
+    _refused(ops._lib().ss_sample_rows(ops._Sample(**d), 0, None), "n_rows")
+    # keys are cut only where a workgroup per query row is a grid
+    b = _batch(n_tokens=1 << 20, max_new=1, n_seqs=1)
+    need = lambda heads: ops._lib().ss_kv_attention_workspace(_cache(n_kv_heads=1, page_stride=256 * 64, page_size=256), b, heads)  # noqa: E731
+    b.max_pages, b.table_stride, b.max_len = 64, 64, 0
+    assert need(8) > 0 and need(16) == 0
