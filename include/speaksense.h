@@ -417,7 +417,7 @@ int ss_kv_read(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_r
  * ones among them.  Query head i reads key head i / (n_heads / n_kv_heads).  causal != 0: a token sees the positions up to its own; 0: all kv_len of
  * them (cross-attention).  Keys on no page are not seen.  A token that sees no key gets zeros (lse -inf).  Rows of pages behind kv_len may hold anything; keys
  * and values that some token of the sequence sees are taken to be finite.
- * out: as q.  lse (optional): float32 [n_tokens][n_heads], the natural logarithm of the softmax's denominator, with which results over disjoint keys
+ * out: as q, not overlapping it or the cache.  lse (optional): float32 [n_tokens][n_heads], the natural logarithm of the softmax's denominator, with which results over disjoint keys
  * are joined.  Softmax and sums are held in float32; the probabilities are rounded to the type that the matrix product takes (dtype; f16 for 8-bit
  * caches, whose codes it holds exactly).  Results do not depend on the run, but the order of their sums does on max_new, max_len and n_seqs.
  * workspace: ss_kv_attention_workspace(...) bytes, 16-byte aligned, NULL if that is 0; contents before and after mean nothing. */

@@ -9,6 +9,11 @@
 // 2048 equal steps of the logit finds the step in which the target is crossed, the ids of that step are gathered into LDS and ranked there exactly by
 // (logit, id).  A step that holds more ids than the list (equal or crowded logits) is cut again by the bits of its keys until the ids fit or are all
 // equal; equal ids are then taken in the order of their number.
+//
+// Passes over the row, which stays in L2 after the first: the largest logit; k up to 512: one more for the ids above a bound; other k and top_p: the histogram and
+// the step's ids; a row that a list does not hold: the kept weights.  Bound by the vector instructions of those passes (the double exponential and the LDS
+// atomic of an id are some 40 of them), for few rows by the chain of barriers: 51866 float32 logits, 1 row 21 us, 160 rows without a filter 26, with k = 40 26, with
+// top_p 0.9 at t = 1 58 (mixed settings 54: 620 GB/s), 512 rows of 128000 bfloat16 85 without a filter (1.5 TB/s), mixed 145.
 #include <algorithm>
 #include <type_traits>
 
@@ -129,7 +134,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
 
     // f(group, first id of the lane, its VEC logits) over the wave's groups, the loads of the next AHEAD groups in flight.  f appears once in a rolled
     // loop: a workgroup runs through its code only a few times, and instruction fetches cost more than the moves between the buffers.
-    // (inlined by force, as the passes below: a call keeps this kernel's variables in memory, 61 against 42 us for a row)
+    // (inlined by force, as the passes below: a call keeps this kernel's variables in memory, 55 us for one row of 128000 instead of 35)
     auto over_row = [&](auto f) __attribute__((always_inline)) {
         typename R::V v[AHEAD];
 #pragma unroll

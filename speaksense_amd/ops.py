@@ -2,7 +2,8 @@
 new tokens over it, and filtered sampling of logits.
 
 Calls launch on torch's current stream of the tensors' device and return at once; results and workspaces come from torch's allocator, so calls
-can be captured into a graph.  Wrong arguments raise ValueError (or SpeakSenseError from the library) before anything is launched."""
+can be captured into a graph.  Wrong arguments raise ValueError (or SpeakSenseError from the library) before anything is launched.  The operators serve: they
+have no gradients, and inputs that ask for one are refused (use torch.no_grad() or detach())."""
 from __future__ import annotations
 
 import ctypes as C
@@ -151,9 +152,15 @@ class KvBatch:
         self._c = _Batch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride, n, pages, n_tokens, max_new, min_new, max_len)
 
 
+def _no_gradient(t, name):
+    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which this operator does not have")
+
+
 def _rows(t, name, cache, batch, heads):
     """The C view of token rows [n_tokens, heads, head_dim]; `heads` None: any number."""
     if isinstance(t, torch.Tensor) and t.dtype is cache.dtype and t.get_device() == cache.index:
+        if t.requires_grad:
+            _no_gradient(t, name)
         shape = t.shape
         if len(shape) == 3 and shape[0] == batch.n_tokens and shape[2] == cache.head_dim and (heads is None or shape[1] == heads):
             row, head, element = t.stride()
@@ -221,6 +228,7 @@ def sample_rows(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
     """One id per row of logits [n_rows, n_vocab] (float32, float16 or bfloat16) from uniform numbers u [n_rows] (float64): temperature, top-k, top-p and
     min-p per row (ss_sample_rows).  Each setting is a tensor [n_rows] (float32; top_k int32) on the device, or None for "off"."""
     _on(logits, None, "logits")
+    _no_gradient(logits, "logits")
     dev, index = logits.device, logits.get_device()
     _need(logits.dtype in _DTYPES, f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
     _need(logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1), "logits must be [n_rows, n_vocab] with contiguous rows")

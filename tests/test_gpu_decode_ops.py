@@ -181,3 +181,19 @@ def test_rows_of_the_engine_rules(toy_ml_path):
     for _ in range(4):
         got = ops.sample_rows(x.cuda(), torch.from_numpy(rng.random(n)).cuda()).id.cpu().long()
         assert math.isfinite(float(x.gather(1, got[:, None]).min()))
+
+
+def test_inputs_that_ask_for_a_gradient_are_refused():
+    cache = ops.KvCache.empty(1, 1, 16, 64)
+    t32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    b = ops.KvBatch(t32(0)[None], t32(0, 1), t32(1), n_tokens=1, max_new=1)
+    x = torch.ones((1, 1, 64), dtype=torch.float16, device="cuda")
+    g = x.clone().requires_grad_()
+    rows = torch.zeros((1, 9), device="cuda", requires_grad=True)
+    u = torch.zeros(1, dtype=torch.float64, device="cuda")
+    for call in (lambda: ops.kv_append(cache, b, g, x), lambda: ops.kv_append(cache, b, x, g), lambda: ops.kv_attention(cache, b, g), lambda: ops.sample_rows(rows, u)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(ops.kv_attention(cache, b, g.detach()), x)
