@@ -14,6 +14,20 @@ namespace {
 
 constexpr int kFrameThreads = 256;
 
+// one rounding each.  __fmul_rn() and the like are plain operators that the compiler fuses; which of them it left alone hung on the packed instructions it chose
+__device__ __forceinline__ float mul_rn(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+__device__ __forceinline__ float add_rn(float a, float b) {
+#pragma clang fp contract(off)
+    return a + b;
+}
+__device__ __forceinline__ float sub_rn(float a, float b) {
+#pragma clang fp contract(off)
+    return a - b;
+}
+
 __device__ __forceinline__ float padded_sample(const float* pcm, int n, long i) {
     // sp[i]: 200 reflected samples, the audio, then zeros (30 s + 200)
     if (i < 200) return n > 200 ? pcm[200 - i] : 0.0f;
@@ -40,7 +54,7 @@ __global__ __launch_bounds__(kFrameThreads) void mel_frame_kernel(MelTables mt, 
     for (int i = tid; i < 400; i += kFrameThreads) {
         s_sin[i] = mt.sin_t[i];
         s_cos[i] = mt.cos_t[i];
-        s_in[i] = __fmul_rn(mt.hann[i], padded_sample(pcm, n_samples, (long)frame * kHop + i));
+        s_in[i] = mul_rn(mt.hann[i], padded_sample(pcm, n_samples, (long)frame * kHop + i));
     }
     __syncthreads();
     // stage 0: 16 DFT-25 leaves; leaf r holds x[16 n + r]; F0[r][k] at s_a[(r*25 + k)*2]
@@ -50,8 +64,8 @@ __global__ __launch_bounds__(kFrameThreads) void mel_frame_kernel(MelTables mt, 
         for (int n = 0; n < 25; n++) {
             const int idx = (k * n * 16) % 400;
             const float x = s_in[16 * n + r];
-            re = __fadd_rn(re, __fmul_rn(x, s_cos[idx]));
-            im = __fsub_rn(im, __fmul_rn(x, s_sin[idx]));
+            re = add_rn(re, mul_rn(x, s_cos[idx]));
+            im = sub_rn(im, mul_rn(x, s_sin[idx]));
         }
         s_a[2 * t] = re;
         s_a[2 * t + 1] = im;
@@ -72,10 +86,10 @@ __global__ __launch_bounds__(kFrameThreads) void mel_frame_kernel(MelTables mt, 
             const float er = E[0], ei = E[1], re_odd = O[0], im_odd = O[1];
             float* o0 = dst + 2 * (rho * N + k);
             float* o1 = dst + 2 * (rho * N + k + h);
-            o0[0] = __fsub_rn(__fadd_rn(er, __fmul_rn(re, re_odd)), __fmul_rn(im, im_odd));
-            o0[1] = __fadd_rn(__fadd_rn(ei, __fmul_rn(re, im_odd)), __fmul_rn(im, re_odd));
-            o1[0] = __fadd_rn(__fsub_rn(er, __fmul_rn(re, re_odd)), __fmul_rn(im, im_odd));
-            o1[1] = __fsub_rn(__fsub_rn(ei, __fmul_rn(re, im_odd)), __fmul_rn(im, re_odd));
+            o0[0] = sub_rn(add_rn(er, mul_rn(re, re_odd)), mul_rn(im, im_odd));
+            o0[1] = add_rn(add_rn(ei, mul_rn(re, im_odd)), mul_rn(im, re_odd));
+            o1[0] = add_rn(sub_rn(er, mul_rn(re, re_odd)), mul_rn(im, im_odd));
+            o1[1] = sub_rn(sub_rn(ei, mul_rn(re, im_odd)), mul_rn(im, re_odd));
         }
         __syncthreads();
         float* t2 = src; src = dst; dst = t2;
@@ -83,7 +97,7 @@ __global__ __launch_bounds__(kFrameThreads) void mel_frame_kernel(MelTables mt, 
     // power spectrum for bins 0..200 into dst (reuse as real array)
     for (int k = tid; k < kNBins; k += kFrameThreads) {
         const float a = src[2 * k], b = src[2 * k + 1];
-        dst[k] = __fadd_rn(__fmul_rn(a, a), __fmul_rn(b, b));
+        dst[k] = add_rn(mul_rn(a, a), mul_rn(b, b));
     }
     __syncthreads();
     float vmax = -1e30f;
@@ -92,13 +106,13 @@ __global__ __launch_bounds__(kFrameThreads) void mel_frame_kernel(MelTables mt, 
         double sum = 0.0;
         int k = 0;
         for (; k < kNBins - 3; k += 4) {
-            float part = __fmul_rn(dst[k], fl[k]);
-            part = __fadd_rn(part, __fmul_rn(dst[k + 1], fl[k + 1]));
-            part = __fadd_rn(part, __fmul_rn(dst[k + 2], fl[k + 2]));
-            part = __fadd_rn(part, __fmul_rn(dst[k + 3], fl[k + 3]));
+            float part = mul_rn(dst[k], fl[k]);
+            part = add_rn(part, mul_rn(dst[k + 1], fl[k + 1]));
+            part = add_rn(part, mul_rn(dst[k + 2], fl[k + 2]));
+            part = add_rn(part, mul_rn(dst[k + 3], fl[k + 3]));
             sum += (double)part;
         }
-        for (; k < kNBins; k++) sum += (double)__fmul_rn(dst[k], fl[k]);
+        for (; k < kNBins; k++) sum += (double)mul_rn(dst[k], fl[k]);
         sum = log10(sum > 1e-10 ? sum : 1e-10);
         const float v = (float)sum;
         mel[(size_t)j * n_len + frame] = v;
@@ -172,7 +186,7 @@ __global__ __launch_bounds__(kEnergyBlock) void signal_energy_kernel(const float
     if (i >= n) return;
     float sum = 0.0f;
 #pragma unroll
-    for (int j = 0; j <= 2 * kEnergyHw; j++) sum = __fadd_rn(sum, ax[threadIdx.x + j]);
+    for (int j = 0; j <= 2 * kEnergyHw; j++) sum = add_rn(sum, ax[threadIdx.x + j]);
     e[i] = __fdiv_rn(sum, (float)(2 * kEnergyHw + 1));
 }
 
