@@ -228,7 +228,11 @@ __device__ __forceinline__ void f8_epilogue(const GemmF8Desc& g, f32x16 (&acc)[2
                     const int bb = (int)(m / g.rows_per_batch), t = (int)(m % g.rows_per_batch);
                     V4 o;
 #pragma unroll
-                    for (int r = 0; r < 4; r++) o[r] = (T)acc[ni][mi][gq * 4 + r];
+                    for (int r = 0; r < 4; r++) {
+                        float v = acc[ni][mi][gq * 4 + r];
+                        asm("" : "+v"(v));     // float32 first, as the plain rows have it: fused with the scale and the bias (v_fma_mix) it would be rounded once
+                        o[r] = (T)v;
+                    }
                     *(V4*)((T*)g.out + (((long)(bb * H + h) * 64 + j) * g.Tpad + t)) = o;
                 }
         }
