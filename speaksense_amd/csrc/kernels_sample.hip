@@ -298,7 +298,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     auto alive = [&](float x, int id) { return x > thr || (x == thr && id <= thr_id); };
     // (a span beyond 64 is the work of a mask of some lowest number: the histogram's steps are for the logits above it.
     // With 2 % of the ids at float32's lowest and steps up to it, k = 40 of 160 rows took 141 us instead of 26)
-    low = fmaxf(low, top - 64.0f);
+    low = low < top ? fmaxf(low, top - 64.0f) : top - 64.0f;              // (the sample may be all masked)
     const float steps = low < top ? (float)(kBins - 1) / (top - low) : 0.0f;
     auto bin_of = [&](float x) { return (int)fminf(fmaxf((top - x) * steps, 0.0f), (float)(kBins - 1)); };   // NaN: 0
     auto value_of = [&](unsigned key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); };

@@ -262,3 +262,13 @@ def test_long_lists_and_wide_nuclei():
         x[6, 100:2000] = x[6].max()                                     # more best ids than the list holds
         u = torch.rand((8,), generator=g, dtype=torch.float64).tolist()
         check(x, u, t=[1.0, 1.0, 3.0, 2.0, 1.0, 4.0, 1.0, 2.0], k=[511, 512, 513, 1500, 20000, 0, 700, 0], p=[1.0, 0.9, 1.0, 0.99, 1.0, 0.97, 0.5, 0.9])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_rows_whose_first_ids_are_masked(dt):
+    """As under a rule that leaves only the last ids of the vocabulary: nothing of what comes first says how the logits are spread."""
+    g = torch.Generator().manual_seed(14)
+    x = (torch.randn((8, 20000), generator=g) * 2.5).to(dt)
+    x[:, :18500] = -math.inf
+    u = torch.rand((8,), generator=g, dtype=torch.float64).tolist()
+    check(x, u, t=[1.0] * 8, k=[0, 40, 0, 600, 1, 1499, 0, 5], p=[1.0, 1.0, 0.9, 1.0, 1.0, 0.95, 0.5, 0.7], m=[0.0] * 6 + [0.05] * 2)
