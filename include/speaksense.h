@@ -419,7 +419,8 @@ int ss_kv_read(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_r
  * and values that some token of the sequence sees are taken to be finite.
  * out: as q, not overlapping it or the cache.  lse (optional): float32 [n_tokens][n_heads], the natural logarithm of the softmax's denominator, with which results over disjoint keys
  * are joined.  Softmax and sums are held in float32; the probabilities are rounded to the type that the matrix product takes (dtype; f16 for 8-bit
- * caches, whose codes it holds exactly).  Results do not depend on the run, but the order of their sums does on max_new, max_len and n_seqs.
+ * caches, whose codes it holds exactly).  In an 8-bit cache each token's terms probability * scale are rounded relative to the largest that this token sees, so
+ * value rows may differ in size by 2^120 within a sequence.  Results do not depend on the run, but the order of their sums does on max_new, max_len and n_seqs.
  * workspace: ss_kv_attention_workspace(...) bytes, 16-byte aligned, NULL if that is 0; contents before and after mean nothing. */
 int64_t ss_kv_attention_workspace(const ss_kv_cache* cache, const ss_kv_batch* batch, int32_t n_heads);   /* < 0: SS_ERR_ARG.  Host only */
 int ss_kv_attention(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_rows* q, int32_t n_heads, float scale, int32_t causal, const ss_kv_rows* out,

@@ -254,11 +254,17 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, int shift, T* __
 // little block with v_perm: MFMA number jj takes column (D/16) (lane & 15) + jj.  No transposed copy of V exists anywhere.
 //
 // 8-bit caches: codes enter the MFMA as f16 (exact: |code| <= 448) whatever the tokens' type; a key's scale multiplies its score in f32, a value's
-// scale multiplies its probability, relative to a running power of two (sref) near the largest scale seen, so that no term leaves f16's range.
-// bf16 queries are brought to f16 by a power of two of their own (exact but for elements below 2^-24 of the row's largest).
+// scale multiplies its probability, relative to a running power of two (sref) near the largest scale seen, so that no term leaves f16's range at the top.
+// bf16 queries are brought to f16 by a power of two of their own (exact but for elements below 2^-17 of the row's largest, which keep steps of 2^-24 of it).
 //
 // m_q need not be the maximum, only near it: it moves when a score exceeds it by more than 2^8 (p then is at most 2^8, in f16 as in bf16), which
 // leaves most tiles without a reduction across lanes and without rescaling O.
+//
+// At the bottom f16 holds a term p v_j / sref in full only from 2^-14 on, and sref may belong to a key that a row does not see or that weighs nothing there.  So
+// over 8-bit caches all p of a row are taken 2^lift higher (l, O and p alike: the division takes it out): 2^5, and where the row's largest term lies
+// below 2^-8, as much more as brings it to 1, as far as float32 holds p (2^121; l is kept 2^64 lower, so that its sum stays in range too).  Terms then reach
+// 2^(8 + 2 + 5) at most, and the row's largest lies at 2^-3 or above.  It is looked for only where m or sref moved and while some row of the wave is low; in
+// between it can only grow.
 // ---------------------------------------------------------------------------------------------
 struct AttnArgs {
     const void* q; long q_row, q_head;
@@ -273,6 +279,9 @@ struct AttnArgs {
 
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kSlack = 8.0f;         // log2 of the largest probability relative to m
+constexpr float kRefRange = 4.0f;      // of a value's scale above sref
+constexpr float kLift = 5.0f, kLow = -8.0f, kMostLift = 121.0f;     // 8-bit caches, in log2 units
+constexpr float kDown = 0x1p-64f;      // 8-bit caches: on l
 
 template <int KIND> struct Held;       // what the MFMA multiplies, and bytes of an element
 template <> struct Held<K_F16> { typedef f16 M; static constexpr int B = 2; };
@@ -383,18 +392,24 @@ template <typename M, int KIND, int D> struct VBlock {
 
 // Online softmax state of one column tile (a lane's query row), and the step for 32 keys
 template <typename M, bool SCALED, int D> struct Row {
-    float m = -kInf, l = 0.0f;         // m: in log2 units; l: this lane's keys only, summed over the four groups at the end
-    float raw = 0.0f;                  // m before the factor c
+    float raw = -kInf, l = 0.0f;       // m before the factor c; l: this lane's keys only, total() sums the four groups
+    float big = -kInf;                 // SCALED: log2 of the row's largest term p v / sref where it was last looked for, p relative to 2^m
     f32x4 o[D / 16];
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[i] = (f32x4){0, 0, 0, 0};
     }
-    __device__ __forceinline__ void move(float top, float c) {          // m up to the largest score so far, what was summed along with it
-        const float rn = m == -kInf ? rows_max(top) : fmaxf(raw, rows_max(top)), mn = rn * c, ref = mn == -kInf ? 0.0f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        raw = mn == -kInf ? 0.0f : rn;
+    __device__ __forceinline__ float m(float c) const { return raw * c; }        // in log2 units
+    __device__ __forceinline__ float lift() const {          // a whole number; l and o hold 2^lift times the sums relative to 2^m
+        return !SCALED ? 0.0f : big < kLow && big > -kInf ? kLift + fminf(ceilf(-big), kMostLift) : kLift;
+    }
+    __device__ __forceinline__ float unlift() const { return __uint_as_float((unsigned)(127 - (int)lift()) << 23); }
+    __device__ __forceinline__ void sum(float w) { l = SCALED ? fmaf(w, kDown, l) : l + w; }
+    __device__ __forceinline__ float total() const {          // relative to 2^m
+        const float t = rows_sum(l);
+        return SCALED ? t * unlift() * (1.0f / kDown) : t;
+    }
+    __device__ __forceinline__ void scale(float a) {
         l *= a;
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[i] *= a;
@@ -404,40 +419,66 @@ template <typename M, bool SCALED, int D> struct Row {
         for (int i = 0; i < D / 16; i++) o[i] = Mfma<M>::mma(vf[i], p, o[i]);
     }
 };
+struct Gauge { bool far = false, low = false; };       // of some row of the wave: |m| is large; its largest term is small
 
-// Scores x[QC][8] of 32 keys (-inf where masked; c > 0 brings them to log2 units) -> the probabilities' B operands; v[8]: value scales / sref.
+// Scores x[QC][8] of 32 keys (-inf where masked; c > 0 brings them to log2 units) -> what probs() subtracts from x c.  `value(e)`: scale / sref of
+// the key of score e; by: what sref's last move multiplied O by, 1 if it did not move.
 // exp2(x c - m) is one fma and one exponential.  The fma does not round x c where m did, so every probability of the row is off by the factor
 // 2^(x c - m at the maximum), at most 2^(|m| 2^-24), which the division by l takes out again but for what m's moves leave: below 2^-12 of it as far
 // as |m| <= 2^12 (the scores' own float32 steps then are as large).  Beyond that (far, the same for the whole wave) the difference is formed first.
-template <int QC, int NE, typename M, bool SCALED, int D>
-__device__ __forceinline__ void softmax_ref(Row<M, SCALED, D>* st, bool& far, float (*x)[NE], const float* c, float* ref) {
+template <int QC, int NE, typename M, bool SCALED, int D, typename F>
+__device__ __forceinline__ void softmax_ref(Row<M, SCALED, D>* st, Gauge& ga, float by, float (*x)[NE], const float* c, float* ref, F value) {
     float top[QC];
-    bool moved = false;
+    bool moved = SCALED && by != 1.0f;
 #pragma unroll
     for (int j = 0; j < QC; j++) {
         top[j] = x[j][0];
 #pragma unroll
         for (int e = 1; e < NE; e++) top[j] = fmaxf(top[j], x[j][e]);
-        moved |= top[j] * c[j] > st[j].m + kSlack;
-        ref[j] = st[j].m == -kInf ? 0.0f : st[j].m;
+        const float m = st[j].m(c[j]);
+        moved |= top[j] * c[j] > m + kSlack;
+        ref[j] = (m == -kInf ? 0.0f : m) - (SCALED ? kLift : 0.0f);
     }
-    if (__ballot(moved) || far) {
+    if (__ballot(moved) || ga.far || ga.low) {
         asm volatile("");              // a branch, not selects
-        bool f = false;
+        bool f = false, w = false;
 #pragma unroll
-        for (int j = 0; j < QC; j++) {
-            st[j].move(top[j], c[j]);
-            ref[j] = st[j].m == -kInf ? 0.0f : st[j].m;
+        for (int j = 0; j < QC; j++) {                     // m up to the largest score so far, what was summed along with it
+            const float old = st[j].m(c[j]);
+            st[j].raw = fmaxf(st[j].raw, rows_max(top[j]));
+            const float mn = st[j].m(c[j]);
+            ref[j] = mn == -kInf ? 0.0f : mn;
+            st[j].scale(__builtin_amdgcn_exp2f(old - ref[j]) * (SCALED ? st[j].unlift() : 1.0f));
+            if (SCALED) st[j].big += old - ref[j] + __builtin_amdgcn_logf(by);       // by 0: nothing but zeros has been summed
             f |= fabsf(ref[j]) > 4096.0f;
         }
-        far = __ballot(f) != 0;
-        if (far)
+        ga.far = __ballot(f) != 0;
+        if (ga.far)
 #pragma unroll
             for (int j = 0; j < QC; j++) {
 #pragma unroll
-                for (int e = 0; e < NE; e++) x[j][e] -= st[j].raw;
+                for (int e = 0; e < NE; e++) x[j][e] -= st[j].raw == -kInf ? 0.0f : st[j].raw;
                 ref[j] = 0.0f;
             }
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int j = 0; j < QC; j++) top[j] = -kInf;
+#pragma unroll
+            for (int e = 0; e < NE; e++) {
+                const float v = __builtin_amdgcn_logf(value(e));
+#pragma unroll
+                for (int j = 0; j < QC; j++) top[j] = fmaxf(top[j], fmaf(x[j][e], c[j], v - ref[j]));
+            }
+#pragma unroll
+            for (int j = 0; j < QC; j++) {
+                st[j].big = fmaxf(st[j].big, rows_max(top[j]));
+                w |= st[j].raw > -kInf && st[j].big < kLow;
+                const float lift = st[j].lift();
+                st[j].scale(__uint_as_float((unsigned)(127 + (int)lift) << 23));
+                ref[j] -= lift;
+            }
+            ga.low = __ballot(w) != 0;
+        }
     }
 }
 // 8 scores of a lane -> its B operand
@@ -447,7 +488,7 @@ __device__ __forceinline__ typename Mfma<M>::V8 probs(Row<M, SCALED, D>& st, con
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         const float w = __builtin_amdgcn_exp2f(fmaf(x[e], c, -ref));
-        st.l += w;
+        st.sum(w);
         p[e] = (M)(SCALED ? w * v[e] : w);
     }
     return p;
@@ -458,9 +499,9 @@ struct ScaleRef {
     float ref = 0.0f;
     // of the scales of a tile, `top` the lane's largest: did it move, and what O has to be multiplied by then
     __device__ __forceinline__ bool moves(float top, float* by) {
-        if (!__ballot(top > ref * 64.0f)) return false;
-        const float n = __uint_as_float(__float_as_uint(fmaxf(wave_max(top), ref)) & 0x7f800000u);
-        *by = n > 0.0f ? ref / n : 0.0f;
+        if (!__ballot(top > ref * kRefRange)) return false;
+        const float n = fmaxf(__uint_as_float(__float_as_uint(fmaxf(wave_max(top), ref)) & 0x7f800000u), 1.17549435e-38f);   // (scales may be subnormal)
+        *by = ref / n;
         ref = n;
         return true;
     }
@@ -542,7 +583,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
     constexpr bool SCALED = Held<KIND>::B == 1;
     constexpr int N = D / 16;
     __shared__ float s_o[4][16][D];
-    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ float s_m[4][16], s_l[4][16], s_ref[4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int h = blockIdx.y, s = blockIdx.x / t.splits, split = blockIdx.x % t.splits;
     const Span sp = seq_span(a, s);
@@ -561,7 +602,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
     const int n = hi > lo ? (hi - lo + 31) / 32 : 0, mine_n = n > wave ? (n - wave + 3) / 4 : 0;   // tiles of the range / of this wave
     Row<M, SCALED, D> st;
     st.clear();
-    bool far = false;
+    Gauge ga;
     ScaleRef sr;
 
     int ids[2] = {-1, -1};             // lane i: the pages of this wave's tile i of the current 64
@@ -611,8 +652,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
                 }
             }
         }
+        float by = 1.0f;
         if constexpr (SCALED) {
-            float by;
             const float* v = x.vs;
             if (sr.moves(fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]))), &by))
 #pragma unroll
@@ -622,7 +663,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
             for (int j = 0; j < 8; j++) x.vs[j] *= inv;
         }
         float m;
-        softmax_ref<1, 8>(&st, far, &sc, &c2, &m);
+        softmax_ref<1, 8>(&st, ga, by, &sc, &c2, &m, [&](int e) { return x.vs[e]; });
         const V8 p = probs(st, sc, c2, m, x.vs);
         V8 vf[N];
         x.v.frags(vf);
@@ -639,16 +680,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
         }
     }
 
-    // merge the four waves
-    const float l = rows_sum(st.l);
-    if (lane < 16) { s_m[wave][c] = st.m; s_l[wave][c] = l; }
+    // merge the four waves: sums relative to the largest m and, in 8 bits, to the largest sref (of 0 where a wave met no value but zeros)
+    const float l = st.total();
+    const float m = st.m(c2);
+    if (lane < 16) { s_m[wave][c] = m; s_l[wave][c] = l; }
+    if (SCALED && lane == 0) s_ref[wave] = sr.ref;
     __syncthreads();
+    const float R = SCALED ? fmaxf(fmaxf(s_ref[0], s_ref[1]), fmaxf(s_ref[2], s_ref[3])) : 1.0f;
     float M4 = fmaxf(fmaxf(s_m[0][c], s_m[1][c]), fmaxf(s_m[2][c], s_m[3][c]));
-    const float f = __builtin_amdgcn_exp2f(st.m - M4) * (SCALED ? sr.ref : 1.0f);
+    const float f = __builtin_amdgcn_exp2f(m - M4) * (SCALED && R > 0.0f ? sr.ref / R : 1.0f);
 #pragma unroll
     for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int k = 0; k < N; k++) s_o[wave][c][N * (4 * g + r) + k] = M4 == -kInf ? 0.0f : st.o[k][r] * f;
+        for (int k = 0; k < N; k++) s_o[wave][c][N * (4 * g + r) + k] = M4 == -kInf ? 0.0f : st.o[k][r] * st.unlift() * f;
     __syncthreads();
     const int oc = threadIdx.x >> 4, col = (threadIdx.x & 15) * N;
     if (oc >= rows) return;
@@ -663,13 +707,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
     if (t.splits == 1) {
         const float inv = L > 0.0f ? 1.0f / L : L;         // no key: zeros (L is 0 or NaN here)
 #pragma unroll
-        for (int k = 0; k < N; k++) acc[k] *= inv;
+        for (int k = 0; k < N; k++) acc[k] = acc[k] * inv * R;       // (in this order: R may be the smallest normal number)
         store_cols<T, N>((T*)t.out + (long)orow * t.o_row + (long)ohead * t.o_head + col, acc);
         if (t.lse && col == 0) t.lse[at] = L > 0.0f ? (M4 + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
     } else {
         float* o = t.part + (at * t.splits + split) * D + col;
 #pragma unroll
-        for (int k = 0; k < N; k++) o[k] = acc[k];
+        for (int k = 0; k < N; k++) o[k] = acc[k] * R;
         if (col == 0) t.part_ml[at * t.splits + split] = make_float2(M4, L);
     }
 }
@@ -689,7 +733,8 @@ template <typename M> __device__ __forceinline__ typename Mfma<M>::V8 read_tr(co
 }
 
 template <typename T, int KIND, int D, int QC>
-__global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs t) {
+// (launch bounds: head_dim 64 with two column tiles at 3 waves a SIMD, 168 registers of the 172 that it would take)
+__global__ __launch_bounds__(256, D == 64 && QC == 2 ? 3 : 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs t) {
     typedef typename Held<KIND>::M M;
     typedef typename Mfma<M>::V8 V8;
     constexpr bool SCALED = Held<KIND>::B == 1;
@@ -822,14 +867,15 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     };
     int hole = 0;                      // `bad` of the tile that is computed
     const int koff = c * KP + g * 16, voff = 64 * KP + (4 * g + (c >> 2)) * VP + (c & 3) * 8;
-    bool far = false;
+    Gauge ga;
     float ref = 1.0f;                  // sref of what this wave has summed
     auto compute = [&](bool edge, const char* buf, int key0) {      // edge: some key of the tile is masked for some row of the wave
         const float* sc = (const float*)(buf + 64 * (KP + VP));
+        float by = 1.0f;
         if constexpr (SCALED) {
             ref = sc[128];
-            const float by = sc[129];
-            if (__builtin_amdgcn_readfirstlane(__float_as_int(by)) != __float_as_int(1.0f))
+            by = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sc[129])));
+            if (by != 1.0f)
 #pragma unroll
                 for (int j = 0; j < QC; j++)
 #pragma unroll
@@ -883,7 +929,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
             }
         }
         float m[QC];
-        softmax_ref<QC, 16>(st, far, x, c2, m);
+        softmax_ref<QC, 16>(st, ga, by, x, c2, m, [&](int e) { return sc[64 + 16 * (e >> 2) + 4 * g + (e & 3)]; });
         float vs[2][8];
         if constexpr (SCALED)
 #pragma unroll
@@ -933,20 +979,20 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
     }
 #pragma unroll
     for (int j = 0; j < QC; j++) {
-        const float L = rows_sum(st[j].l), mm = st[j].m;
+        const float L = st[j].total(), mm = st[j].m(c2[j]);
         if (w0 + 16 * j + c >= rows) continue;
         int head;
         const int row = row_of(j, &head);
         const long at = (long)row * (a.H * t.G) + head;
-        const float u = SCALED ? ref : 1.0f;
+        const float u = SCALED ? ref : 1.0f, un = st[j].unlift();
         if (t.splits == 1) {
-            const float inv = (L > 0.0f ? 1.0f / L : L) * u;
+            const float inv = L > 0.0f ? 1.0f / L : L;
             T* o = (T*)t.out + (long)row * t.o_row + (long)head * t.o_head;
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 float y[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = L == 0.0f ? 0.0f : st[j].o[k][r] * inv;
+                for (int r = 0; r < 4; r++) y[r] = L == 0.0f ? 0.0f : st[j].o[k][r] * un * inv * u;
                 store_cols<T, 4>(o + 16 * k + 4 * g, y);
             }
             if (t.lse && g == 0) t.lse[at] = L > 0.0f ? (mm + __builtin_amdgcn_logf(L)) * 0.69314718055994530942f : (L == 0.0f ? -kInf : L);
@@ -955,7 +1001,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs
 #pragma unroll
             for (int k = 0; k < N; k++) {
                 f32x4 y = {0, 0, 0, 0};
-                if (L != 0.0f) y = st[j].o[k] * u;
+                if (L != 0.0f) y = st[j].o[k] * un * u;
                 *(f32x4*)(o + 16 * k + 4 * g) = y;
             }
             if (g == 0) t.part_ml[at * t.splits + split] = make_float2(mm, L);

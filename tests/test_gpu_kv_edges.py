@@ -1,0 +1,127 @@
+"""GPU: paged-cache operators where the inputs' sizes lie far apart, and where lengths on the device and numbers of the host disagree.
+
+Attention is held to the formula in 64 bits with a bound that looks only at the keys a row sees:
+    |o - o64| <= h_out |o| + (h_p + 2^-15) A + n 2^-21 max_j(p_j amax_j) / l + half a subnormal step of the result's type
+h_out, h_p, A, l as in test_gpu_kv_ops.py.  The third term is f16's subnormal terms: each is off by at most 2^-25, the row's largest term p_j s_j (s_j a value row's
+scale) is held at 2^-3 or above, a code weighs at most amax_j / s_j <= 448, and amax_j > 224 s_j: 2^-25 2^3 2 = 2^-21 of max_j(p_j amax_j) a key."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from speaksense_amd import ops  # noqa: E402
+from test_gpu_kv_ops import DT, Step, quantise  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+KINDS8 = ["e4m3", "int8"]
+
+
+def attend_seen(st, q, scale, causal):
+    """CPU, 64 bits: result and its bound of the rows that a sequence owns."""
+    groups = q.shape[1] // st.heads
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    half_out = torch.finfo(st.dt).eps / 2
+    half_p = torch.finfo(torch.bfloat16 if st.kind == "same" and st.dt == torch.bfloat16 else torch.float16).eps / 2
+    step = torch.finfo(st.dt).tiny * half_out
+    for s in range(len(st.lens)):
+        a, b = st.starts[s], st.starts[s + 1]
+        k, v = st.dense(s, "k").double(), st.dense(s, "v").double()
+        pos = torch.arange(st.lens[s] - (b - a), st.lens[s])
+        seen = torch.arange(st.lens[s])[None] <= pos[:, None] if causal else torch.ones(b - a, st.lens[s], dtype=torch.bool)
+        for h in range(q.shape[1]):
+            x = torch.where(seen, (q[a:b, h].double() @ k[:, h // groups].t()) * scale, -math.inf)
+            p = torch.exp(x - x.amax(-1, keepdim=True))
+            l, w = p.sum(-1, keepdim=True), v[:, h // groups]
+            out[a:b, h] = p @ w / l
+            most = (p * w.abs().amax(-1)).amax(-1, keepdim=True)
+            tol[a:b, h] = half_out * out[a:b, h].abs() + (half_p + 2.0 ** -15) * (p @ w.abs() / l) + seen.sum(-1, keepdim=True) * 2.0 ** -21 * most / l + step
+    return out, tol
+
+
+def refill(st, k, v):
+    """New contents of a Step's cache: float32 rows [n_pages, heads, page, dim]."""
+    k, v = k.to(st.dt), v.to(st.dt)
+    if st.kind == "same":
+        st.k, st.v = k, v
+    else:
+        (st.k, st.ks), (st.v, st.vs) = quantise(k, st.kind), quantise(v, st.kind)
+
+
+def scored_step(lens, new, dim, kind, dt, seed=0):
+    """Keys that score 0.3 randn, and a way to give a position a score and its value row a size."""
+    st = Step(lens, [new] * len(lens), 1, dim, 16, kind, dt, seed=seed)
+    k = torch.randn(st.k.shape, generator=st.g) * 0.3
+    k[..., 0] = 0
+    v = torch.randn(st.k.shape, generator=st.g)
+    q = (torch.randn((st.n, 3, dim), generator=st.g) * 0.3).to(st.dt)
+    q[..., 0] = 4.0
+
+    def put(s, pos, log2_score, log2_size):
+        pg, r = int(st.table[s, pos // 16]), pos % 16
+        k[pg, 0, r, 0] = log2_score * math.log(2.0) * dim ** 0.5 / 4.0
+        v[pg, 0, r] *= 2.0 ** log2_size
+
+    return st, k, v, q, put
+
+
+def hold(st, q, causal=True):
+    st.cuda()
+    want, tol = attend_seen(st, q, st.dim ** -0.5, causal)
+    got = ops.kv_attention(st.cache, st.batch, q.cuda(), causal=causal).cpu().double()
+    over = (got - want).abs() - tol
+    assert not torch.isnan(got).any() and float(over.max()) <= 0, (float(over.max()), int((over > 0).sum()), over.numel())
+
+
+# new tokens a sequence and its lengths: the few-row kernel, the tile kernel, either with its keys cut
+SHAPES = [(1, [180, 333]), (40, [180, 333]), (1, [3000, 65]), (40, [2500])]
+
+
+@pytest.mark.parametrize("kind", KINDS8)
+@pytest.mark.parametrize("dt,gap,base", [("bf16", 24, 0), ("bf16", 60, -30), ("f16", 20, -8)])
+@pytest.mark.parametrize("new,lens", SHAPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_far_below_the_largest(kind, dt, gap, base, new, lens, dim):
+    """Value rows 2^gap times the others: one that only the last token sees; one that all see and that weighs little or as much as the rest; one small row of nearly
+    all weight among them."""
+    for low in (0, 30):
+        st, k, v, q, put = scored_step(lens, new, dim, kind, dt)
+        v *= 2.0 ** base
+        for s, n in enumerate(lens):
+            put(s, n - 1, 0, gap)                          # the last position
+        refill(st, k, v)
+        hold(st, q)
+        for s, n in enumerate(lens):
+            put(s, n // 3, -gap - low, gap)
+        refill(st, k, v)
+        hold(st, q)
+        hold(st, q, causal=False)
+    st, k, v, q, put = scored_step(lens, new, dim, kind, dt)
+    v *= 2.0 ** (base + gap)
+    for s, n in enumerate(lens):
+        put(s, 1, 20, -gap)
+    refill(st, k, v)
+    hold(st, q)
+
+
+@pytest.mark.parametrize("kind", KINDS8)
+@pytest.mark.parametrize("new,lens", SHAPES)
+def test_values_of_subnormal_scales(kind, new, lens):
+    """bfloat16 values near the smallest normal number: an int8 row's scale then is subnormal, an e4m3 row's the smallest there is."""
+    st, k, v, q, put = scored_step(lens, new, 64, kind, "bf16")
+    refill(st, k, v * 2.0 ** -122)
+    hold(st, q)
+
+
+@pytest.mark.parametrize("kind", KINDS8)
+@pytest.mark.parametrize("new", [1, 40])
+def test_values_that_rise_and_fall_along_the_keys(kind, new):
+    """Sizes that grow by 2^2 every few keys, against falling scores, and the other way round: the running scale moves in most tiles, and each row's largest term with it."""
+    for up in (1, -1):
+        st, k, v, q, put = scored_step([300, 140], new, 64, kind, "bf16")
+        for s, n in enumerate(st.lens):
+            for p in range(n):
+                put(s, p, -up * (p // 5) * 2 if p % 7 else 0, up * (p // 5) * 2 - (0 if up > 0 else -60))
+        refill(st, k, v)
+        hold(st, q)
