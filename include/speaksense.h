@@ -394,7 +394,8 @@ typedef struct ss_kv_batch {      /* the sequences of one step */
     int32_t n_seqs;
     int32_t max_pages;            /* max_pages * page_size < 2^30 */
     int32_t n_tokens;             /* rows of the token tensors, <= 2^24 */
-    int32_t max_new;              /* at least the longest span (what a scheduler knows on the host): ss_kv_attention covers max_new tokens per sequence */
+    int32_t max_new;              /* at least the longest span (what a scheduler knows on the host): ss_kv_attention computes the first max_new tokens of a
+                                     span and leaves the results of those behind them as they were; append and read take every token */
     int32_t min_new;              /* the shortest span, or 0 if unknown: a hint, of no effect where the kernels take any mixture as fast (as they do) */
     int32_t max_len;              /* about the longest kv_len, or 0 if unknown: decides only how the keys are cut over workgroups */
 } ss_kv_batch;

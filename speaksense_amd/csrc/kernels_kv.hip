@@ -274,6 +274,7 @@ struct AttnArgs {
     float c2;                          // |scale| * log2(e), at least the smallest normal number: a masked -inf stays one
     int neg;                           // scale < 0: the queries' signs are turned instead
     int G, causal, splits, split_keys; // query heads per key head; key ranges and their length (a multiple of 128)
+    int max_new;                       // the first max_new tokens of a span are computed: the launch has room for no more, whatever q_start holds by now
     int nq;                            // tile kernel: query tiles per (sequence, head)
 };
 
@@ -523,7 +524,7 @@ template <typename T, int N> __device__ __forceinline__ void store_cols(T* p, co
     }
 }
 
-// ---- few query rows (n_new G <= 16 in every sequence): grid (sequences x splits, key heads); the 4 waves of a workgroup take every fourth 32-key tile of its key
+// ---- few query rows (max_new G <= 16): grid (sequences x splits, key heads); the 4 waves of a workgroup take every fourth 32-key tile of its key
 // range straight from memory into registers (the next tile's loads fly while one is computed) and merge at the end.  HBM-bound: with G <= 16 the
 // MFMA issues of a tile take ~1/10 of the time its bytes need at the card's rate, so the 15 idle columns of a one-head row cost nothing.
 // 4 contexts of 30001..65536 bf16 keys, 8 x 4 heads of 128: 116 us, 6.7 TB/s; 96 x 1500 e4m3 keys, 20 heads of 64: 76 us, 4.9 TB/s; a step of 8 short contexts: 9 us. ----
@@ -587,8 +588,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int h = blockIdx.y, s = blockIdx.x / t.splits, split = blockIdx.x % t.splits;
     const Span sp = seq_span(a, s);
-    const int rows = sp.n_new * t.G;
-    if (rows == 0 || rows > 16) return;
+    const int rows = min(sp.n_new, t.max_new) * t.G;       // <= 16
+    if (rows == 0) return;
 
     const bool mine = c < rows;
     const int tok = c / t.G, row = sp.q0 + (mine ? tok : 0), head = h * t.G + (mine ? c % t.G : 0);
@@ -753,7 +754,7 @@ __global__ __launch_bounds__(256, D == 64 && QC == 2 ? 3 : 2) void kv_attn_tile_
     bid /= t.splits;
     const int h = bid % a.H, s = bid / a.H;
     const Span sp = seq_span(a, s);
-    const int rows = sp.n_new * t.G, r0 = qb * (64 * QC);
+    const int rows = min(sp.n_new, t.max_new) * t.G, r0 = qb * (64 * QC);
     if (rows <= r0) return;
 
     const int w0 = r0 + wave * (16 * QC);                  // this wave's first query row
@@ -1020,7 +1021,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvArgs a, AttnArgs t)
     const int s = find_seq(a.q_start, a.n_seqs, row);
     if (s < 0 || s >= a.n_seqs) return;
     const Span sp = seq_span(a, s);
-    if (row < sp.q0 || row >= sp.q0 + sp.n_new) return;
+    if (row < sp.q0 || row >= sp.q0 + min(sp.n_new, t.max_new)) return;
     const float2 ml = lane < t.splits ? t.part_ml[at * t.splits + lane] : make_float2(-kInf, 0.0f);
     const float m = wave_max(ml.x), f = ml.x == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - m);
     const float L = wave_sum(ml.y * f);
@@ -1147,7 +1148,7 @@ void launch_kv_attention(const ss_kv_cache& c, const ss_kv_batch& b, const ss_kv
     AttnArgs t{};
     t.q = q.p; t.q_row = q.row_stride; t.q_head = q.head_stride;
     t.out = out.p; t.o_row = out.row_stride; t.o_head = out.head_stride;
-    t.lse = lse; t.c2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f); t.neg = scale < 0.0f; t.G = n_heads / c.n_kv_heads; t.causal = causal;
+    t.lse = lse; t.c2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f); t.neg = scale < 0.0f; t.G = n_heads / c.n_kv_heads; t.causal = causal; t.max_new = b.max_new;
     by_type(c, [&](auto tt, auto kind, auto dim) {
         typedef decltype(tt) T;
         constexpr int K = kind.value, D = dim.value;

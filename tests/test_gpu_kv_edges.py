@@ -125,3 +125,37 @@ def test_values_that_rise_and_fall_along_the_keys(kind, new):
                 put(s, p, -up * (p // 5) * 2 if p % 7 else 0, up * (p // 5) * 2 - (0 if up > 0 else -60))
         refill(st, k, v)
         hold(st, q)
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# spans longer than the host's max_new (q_start lies on the device and may change under a captured graph)
+# ---------------------------------------------------------------------------------------------------------------------------------
+def raw_attention(st, q, max_new, max_len, causal=True):
+    """The C call with results filled with 7 and a workspace of NaN."""
+    b = ops.KvBatch(st.batch.page_table, st.batch.q_start, st.batch.kv_len, n_tokens=st.n, max_new=max_new, max_len=max_len)
+    heads, L = q.shape[1], ops._lib()
+    out, lse = torch.full(q.shape, 7.0, dtype=st.dt, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
+    need = L.ss_kv_attention_workspace(st.cache._c, b._c, heads)
+    work = torch.full((need // 4 + 4,), math.nan, device="cuda")
+    rows = lambda t: ops._rows(t, "t", st.cache, b, heads)  # noqa: E731
+    assert L.ss_kv_attention(st.cache._c, b._c, rows(q), heads, st.dim ** -0.5, 1 if causal else 0, rows(out), lse.data_ptr(), work.data_ptr(), need, 0, ops._stream(0)) == 0
+    return out.cpu(), lse.cpu(), need
+
+
+@pytest.mark.parametrize("kind,dt,dim", [("same", "bf16", 64), ("int8", "f16", 128)])
+@pytest.mark.parametrize("max_new,groups", [(1, 1), (1, 2), (3, 5), (2, 20), (33, 2)])      # the last two: the tile kernel
+@pytest.mark.parametrize("lens,news", [([60, 90], [3, 40]), ([3000, 700, 50], [3, 40, 1])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_spans_longer_than_max_new(kind, dt, dim, max_new, groups, lens, news, causal):
+    """Their first max_new tokens are computed, at their positions; results of the rest are left as they were, with and without a cut over the keys."""
+    st = Step(lens, news, 1, dim, 16, kind, dt, extra_rows=2)
+    st.cuda()
+    q = torch.randn((st.n, groups, dim), generator=st.g).to(st.dt)
+    want, tol, wlse = st.attend(q, dim ** -0.5, causal)
+    out, lse, need = raw_attention(st, q.cuda(), max_new, max(lens), causal)
+    assert (need > 0) == (max(lens) > 512)
+    done = torch.zeros(st.n, dtype=torch.bool)
+    for s, n in enumerate(news):
+        done[st.starts[s]:st.starts[s] + min(n, max_new)] = True
+    assert ((out.double() - want).abs() <= tol)[done].all() and ((lse.double() - wlse).abs() <= 2.0 ** -12)[done].all()
+    assert (out[~done] == 7.0).all() and (lse[~done] == 7.0).all()
