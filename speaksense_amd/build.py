@@ -11,7 +11,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libspeaksense_hip.so")
 LIB_W155 = os.path.join(HERE, "libspeaksense_whisper_post154.so")
 SOURCES = ["model.cpp", "kernels_mel.hip", "kernels_gemm.hip", "kernels_gemm_fp8.hip", "kernels_attn.hip", "kernels_misc.hip", "kernels_decode.hip", "kernels_denoise.hip", "kernels_resample.hip", "kernels_kv.hip", "kernels_sample.hip", "engine.cpp", "capi.cpp"]
-HEADERS = ["common.h", "kernels.h", "gemm_common.h", "wave_ops.h", "engine.h", "ops.h", os.path.join("..", "..", "include", "speaksense.h"), os.path.join("..", "..", "include", "whisper_compat.h")]
+HEADERS = ["common.h", "kernels.h", "gemm_common.h", "wave_ops.h", "rounded.h", "engine.h", "ops.h", os.path.join("..", "..", "include", "speaksense.h"), os.path.join("..", "..", "include", "whisper_compat.h")]
 # no packed FP32 instructions: hipcc -O3 makes v_pk_{add,mul,fma}_f32 out of ordinary float code, and some of their forms have given wrong results on this
 # hardware now and then (the host pass warns that it does not know the feature: harmless)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-x", "hip"]

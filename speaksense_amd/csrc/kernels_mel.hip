@@ -6,6 +6,7 @@
 // To stay within 1e-4 of the CPU path in low-energy bins the FFT keeps whisper.cpp's structure and op order:
 // radix-2 decimation in time down to 16 DFT-25 leaves, f32, un-fused multiply/add, sin/cos from a 400-entry table.
 #include "kernels.h"
+#include "rounded.h"
 #include "wave_ops.h"
 
 namespace ss {
@@ -13,20 +14,6 @@ namespace ss {
 namespace {
 
 constexpr int kFrameThreads = 256;
-
-// one rounding each.  __fmul_rn() and the like are plain operators that the compiler fuses; which of them it left alone hung on the packed instructions it chose
-__device__ __forceinline__ float mul_rn(float a, float b) {
-#pragma clang fp contract(off)
-    return a * b;
-}
-__device__ __forceinline__ float add_rn(float a, float b) {
-#pragma clang fp contract(off)
-    return a + b;
-}
-__device__ __forceinline__ float sub_rn(float a, float b) {
-#pragma clang fp contract(off)
-    return a - b;
-}
 
 __device__ __forceinline__ float padded_sample(const float* pcm, int n, long i) {
     // sp[i]: 200 reflected samples, the audio, then zeros (30 s + 200)

@@ -3,9 +3,10 @@
 // (sinc_len 256, cutoff 0.95, linear blend of the two nearest of 256 sub-phases, BlackmanHarris2 window, 4096-sample chunks).
 // The output instants are a sequential f64 recurrence (idx += 1/ratio) that also decides how many samples each chunk yields; the host
 // runs it (a few thousand additions per second of audio) and hands the instants over, so lengths and tap positions are exact.
-// One thread per output sample: two 256-tap dot products with the crate's 8-lane accumulation order.  HBM-light (input read once,
+// One thread per output sample: two 256-tap dot products with the crate's 8-lane accumulation order, every product and sum rounded (rounded.h).  HBM-light (input read once,
 // the 256 KB phase table lives in L2), so no LDS staging.
 #include "kernels.h"
+#include "rounded.h"
 
 namespace ss {
 namespace {
@@ -18,12 +19,12 @@ __device__ __forceinline__ float dot8(const float* __restrict__ x, long g0, cons
         for (int u = 0; u < 8; u++) {
             const long g = g0 + j + u;
             const float v = g >= 0 ? x[g] : 0.0f;     // 2*sinc_len samples of zero history before the stream
-            acc[u] = __fadd_rn(acc[u], __fmul_rn(v, sinc[j + u]));
+            acc[u] = add_rn(acc[u], mul_rn(v, sinc[j + u]));
         }
     }
     float t = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 8; u++) t = __fadd_rn(t, acc[u]);
+    for (int u = 0; u < 8; u++) t = add_rn(t, acc[u]);
     return t;
 }
 
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(256) void resample_kernel(const float* __restrict__
     const long base = (long)chunk_of[k] * kChunk;
     const float p0 = dot8(x, base + i0, sincs + (size_t)sub0 * kTaps);
     const float p1 = dot8(x, base + i1, sincs + (size_t)sub1 * kTaps);
-    y[k] = __fadd_rn(p0, __fmul_rn(frac, __fsub_rn(p1, p0)));
+    y[k] = add_rn(p0, mul_rn(frac, sub_rn(p1, p0)));
 }
 }  // namespace
 
