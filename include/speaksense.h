@@ -409,7 +409,9 @@ int32_t ss_sizeof_kv_batch(void);
 int32_t ss_sizeof_kv_rows(void);
 /* Writes the new tokens' keys and values [n_tokens][n_kv_heads][head_dim] into their pages, in the cache's form.  Tokens whose position does not exist
  * or lies on no page are dropped.  No two tokens of a call may share a position of a page (the program copies a shared page before it
- * writes to it).  A row that holds a NaN or an infinity reads back as such, and in an 8-bit cache it may take the rest of its row with it. */
+ * writes to it).  NaN and infinities read back as such, but in an 8-bit cache a row that holds one loses its other elements (they read as zeros, NaN or coarse
+ * values; with a NaN in an int8 row, or beside one in an e4m3 row, an infinity reads as NaN too).  Rounding may carry a number next to the type's largest past
+ * it: such a code reads as an infinity. */
 int ss_kv_append(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_rows* k, const ss_kv_rows* v, int32_t device, void* stream);
 /* The reverse: fills k and v [n_tokens][n_kv_heads][head_dim] with what the cache holds at the tokens' positions, code * scale in float32 rounded once to
  * dtype.  A whole context is read as kv_len tokens.  Positions that do not exist or lie on no page read as zeros. */

@@ -4,6 +4,8 @@
 //   same   f16 / bf16 as the tokens
 //   e4m3   code = RNE_e4m3(x 2^(127 - e)), e = E8M0 byte with amax / 2^(e - 127) <= 448 (the format of the fp8 engine's cross cache)
 //   int8   s = amax / 127 (IEEE), code = rint(x / s)
+// A row with an infinity (and no NaN): its infinities hold the largest code under the exponent 253 (448 2^126 is an infinity) or the scale s = infinity (code 0
+// of the finite elements times that is a NaN).
 // A sequence s of the step has n_s = q_start[s + 1] - q_start[s] new tokens, the last n_s of its kv_len[s] positions; position p lies in row
 // p % page_size of page page_table[s][p / page_size].  Every index that comes from device memory is checked here before it is used: a page number
 // outside [0, n_pages) holds nothing (its keys are masked, reads give zeros, writes are dropped), spans of q_start outside the token rows are empty.
@@ -152,14 +154,20 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int shift, con
 #pragma unroll
             for (int i = 0; i < 16; i++) { f[i] = (float)x[i >> 3][i & 7]; top = max(top, __float_as_uint(f[i]) & 0x7fffffffu); }
             top = lanes_umax<D / 16>(top);
+            const bool infinite = top == 0x7f800000u;
             u32x4 code;
             char* sc = it.is_v ? a.vs : a.ks;
             const long sat = (long)((unsigned long)(unsigned)page * a.sc_stride) + slot;
             if constexpr (KIND == K_E4M3) {
-                const int e = e8m0_for_amax(__uint_as_float(top));
+                const int e = infinite ? 253 : e8m0_for_amax(__uint_as_float(top));
                 const float m = pow2_neg_of_e8m0(e);
 #pragma unroll
-                for (int i = 0; i < 4; i++) code[i] = pack_e4m3x4(f[4 * i] * m, f[4 * i + 1] * m, f[4 * i + 2] * m, f[4 * i + 3] * m);
+                for (int i = 0; i < 16; i++) f[i] *= m;
+                if (infinite)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) f[i] = fminf(fmaxf(f[i], -448.0f), 448.0f);
+#pragma unroll
+                for (int i = 0; i < 4; i++) code[i] = pack_e4m3x4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
                 if (it.c == 0) sc[sat] = (char)e;
             } else {
                 const float s8 = __uint_as_float(top) / 127.0f, by = s8 > 0.0f ? s8 : 1.0f;
@@ -174,10 +182,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int shift, con
                     y = fmaf(fmaf(-by, y, f[i]), r, y);
                     q[i] = rintf(y);
                 }
-                if (__ballot(!(by > 1e-30f && by < 1e30f))) {    // remainders out of float's range; a NaN
+                if (__ballot(!(s8 < 1e30f) || by < 1e-30f)) {    // remainders out of float's range; an infinity; a NaN
                     asm volatile("");
+                    const bool finite = top < 0x7f800000u;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) q[i] = fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f);
+                    for (int i = 0; i < 16; i++) {
+                        const float whole = fminf(fmaxf(rintf(f[i] / by), -127.0f), 127.0f), end = fabsf(f[i]) < __builtin_huge_valf() ? 0.0f : copysignf(127.0f, f[i]);
+                        q[i] = finite ? whole : end;
+                    }
                 }
                 unsigned b[16];
 #pragma unroll

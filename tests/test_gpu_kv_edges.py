@@ -159,3 +159,36 @@ def test_spans_longer_than_max_new(kind, dt, dim, max_new, groups, lens, news, c
         done[st.starts[s]:st.starts[s] + min(n, max_new)] = True
     assert ((out.double() - want).abs() <= tol)[done].all() and ((lse.double() - wlse).abs() <= 2.0 ** -12)[done].all()
     assert (out[~done] == 7.0).all() and (lse[~done] == 7.0).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------
+# append of infinities
+# ---------------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["same", "e4m3", "int8"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_append_of_infinities(kind, dt, dim):
+    """They read back with their signs, at either end of a row and beside the largest finite numbers; a NaN stays one; rows beside them are what they are without."""
+    st = Step([32], [32], 2, dim, 16, kind, dt)
+    cache, batch = st.cuda()
+    x = st.rows((32, 2, dim))
+    plain = x.clone()
+    inf, nan, big = math.inf, math.nan, torch.finfo(st.dt).max
+    marks = {0: {0: inf}, 3: {dim - 1: -inf}, 4: {0: -inf, 1: inf, 17: -inf, 40: inf}, 9: {5: inf, 6: big, 7: -big}, 10: {8: nan}, 16: {2: nan, 3: inf}, 17: dict.fromkeys(range(dim), -inf)}
+    for t, m in marks.items():
+        for i, v in m.items():
+            x[t, 1, i] = v
+    want = []
+    for y in (plain, x):
+        ops.kv_append(cache, batch, y.cuda(), (-y).cuda())
+        want.append([t.cpu() for t in ops.kv_read(cache, batch)])
+    for sign, without, got in ((1, want[0][0], want[1][0]), (-1, want[0][1], want[1][1])):
+        rest = [t for t in range(32) if t not in marks]
+        assert torch.equal(got[rest], without[rest]) and torch.equal(got[:, 0], without[:, 0])
+        for t, m in marks.items():
+            mixed = nan in m.values() and kind != "same"
+            for i, v in m.items():
+                g = float(got[t, 1, i])
+                assert math.isnan(g) if math.isnan(v) or (mixed and math.isinf(v)) else g == sign * v if math.isinf(v) else True, (t, i, v, g)
+        if kind == "same":
+            assert torch.equal(torch.nan_to_num(got, 7.0), torch.nan_to_num(sign * x, 7.0))
