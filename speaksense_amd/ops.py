@@ -3,7 +3,7 @@ new tokens over it, and filtered sampling of logits.
 
 Calls launch on torch's current stream of the tensors' device and return at once; results and workspaces come from torch's allocator, so calls
 can be captured into a graph.  Wrong arguments raise ValueError (or SpeakSenseError from the library) before anything is launched.  The operators serve: they
-have no gradients, and inputs that ask for one are refused (use torch.no_grad() or detach())."""
+have no gradients, and tensors that ask for one are refused, inputs, settings and the cache's alike (use torch.no_grad() or detach()); so are forward-mode duals."""
 from __future__ import annotations
 
 import ctypes as C
@@ -11,6 +11,7 @@ from numbers import Integral
 from typing import NamedTuple
 
 import torch      # before the library: both must share one HIP runtime, torch's, and the loader keeps the first
+from torch.autograd import forward_ad
 
 from . import binding
 
@@ -73,6 +74,13 @@ def _on(t, device, name):
     _need(device is None or t.device == device, f"{name} is on {t.device}, expected {device}")
 
 
+def _no_gradient(t, name):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which this operator does not have")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward-mode gradient, which this operator does not have")
+
+
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):      # 0.1 us; the public way builds a Stream object for 2
     _stream = torch._C._cuda_getCurrentRawStream
 else:
@@ -110,6 +118,7 @@ class KvCache:
                 _need(t.stride()[1:] == (page, 1) and (n == 1 or t.stride(0) == k_scale.stride(0)), "each page's scales must be contiguous, with one stride between pages")
         self.k, self.v, self.k_scale, self.v_scale, self.dtype, self.device, self.index = k, v, k_scale, v_scale, dtype, k.device, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, heads, page, dim
+        self._real = [(t, name) for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)) if t is not None and t.is_floating_point()]
         # a cache of one page may be a view whose stride says nothing
         page_stride = k.stride(0) if n > 1 else heads * page * dim
         scale_stride = 0 if scales is None else k_scale.stride(0) if n > 1 else heads * page
@@ -152,14 +161,10 @@ class KvBatch:
         self._c = _Batch(page_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), stride, n, pages, n_tokens, max_new, min_new, max_len)
 
 
-def _no_gradient(t, name):
-    _need(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires a gradient, which this operator does not have")
-
-
 def _rows(t, name, cache, batch, heads):
     """The C view of token rows [n_tokens, heads, head_dim]; `heads` None: any number."""
     if isinstance(t, torch.Tensor) and t.dtype is cache.dtype and t.get_device() == cache.index:
-        if t.requires_grad:
+        if t.requires_grad or forward_ad._current_level >= 0:
             _no_gradient(t, name)
         shape = t.shape
         if len(shape) == 3 and shape[0] == batch.n_tokens and shape[2] == cache.head_dim and (heads is None or shape[1] == heads):
@@ -176,6 +181,9 @@ def _rows(t, name, cache, batch, heads):
 def _same_device(cache, batch):
     _need(isinstance(cache, KvCache) and isinstance(batch, KvBatch), "expected a KvCache and a KvBatch")
     _need(batch.index == cache.index, "the batch and the cache are on different devices")
+    for t, name in cache._real:
+        if t.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient(t, name)
 
 
 def kv_append(cache: KvCache, batch: KvBatch, k, v) -> None:
@@ -242,6 +250,8 @@ def sample_rows(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
         if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dt and t.shape == (n,) and t.is_contiguous()):
             _on(t, dev, name)
             raise ValueError(f"{name} must be {dt} [{n}], contiguous")
+        if t.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient(t, name)
         ptr.append(t.data_ptr())
     whole, real = torch.empty((2, n), dtype=torch.int32, device=dev), torch.empty((2, n), dtype=torch.float32, device=dev)
     ids, kept = whole.unbind()

@@ -197,3 +197,48 @@ def test_inputs_that_ask_for_a_gradient_are_refused():
         with torch.no_grad():
             call()
     assert torch.equal(ops.kv_attention(cache, b, g.detach()), x)
+
+
+def test_every_tensor_that_asks_for_a_gradient_is_refused():
+    """Settings of the sampler and tensors of the cache too, in reverse and in forward mode."""
+    from torch.autograd import forward_ad
+    t32 = lambda *x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    b = ops.KvBatch(t32(0)[None], t32(0, 1), t32(1), n_tokens=1, max_new=1)
+    x = torch.ones((1, 1, 64), dtype=torch.float16, device="cuda")
+    h = lambda *s, dtype=torch.float16: torch.zeros(s, dtype=dtype, device="cuda")  # noqa: E731
+    logits, u, one = h(1, 9, dtype=torch.float32), h(1, dtype=torch.float64), h(1, dtype=torch.float32) + 0.5
+
+    def calls(mark):
+        """(call, its tensors of which `mark` changes one)"""
+        for at in range(2):
+            kv = [h(1, 1, 16, 64), h(1, 1, 16, 64)]
+            kv[at] = mark(kv[at])
+            c = ops.KvCache(*kv)
+            sc = [h(1, 1, 16, dtype=torch.float32), h(1, 1, 16, dtype=torch.float32)]
+            sc[at] = mark(sc[at])
+            c8 = ops.KvCache(h(1, 1, 16, 64, dtype=torch.int8), h(1, 1, 16, 64, dtype=torch.int8), *sc, kind="int8", dtype=torch.float16)
+            for cache in (c, c8):
+                yield from (lambda cache=cache: ops.kv_append(cache, b, x, x), lambda cache=cache: ops.kv_read(cache, b), lambda cache=cache: ops.kv_attention(cache, b, x))
+        plain = ops.KvCache(h(1, 1, 16, 64), h(1, 1, 16, 64))
+        m = mark(x.clone())
+        yield from (lambda: ops.kv_append(plain, b, m, x), lambda: ops.kv_append(plain, b, x, m), lambda: ops.kv_attention(plain, b, m), lambda: ops.kv_attention(plain, b, x, out=mark(x.clone())))
+        yield from (lambda: ops.sample_rows(mark(logits.clone()), u), lambda: ops.sample_rows(logits, mark(u.clone())))
+        for name in ("temperature", "top_p", "min_p"):
+            yield lambda name=name: ops.sample_rows(logits, u, **{name: mark(one.clone())})
+
+    n = 0
+    for call in calls(lambda t: t.requires_grad_()):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        n += 1
+    with forward_ad.dual_level():
+        for call in calls(lambda t: forward_ad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            n -= 1
+        ops.sample_rows(logits, u, temperature=one)        # nothing that carries one
+    assert n == 0
+    with torch.no_grad():
+        ops.sample_rows(logits.requires_grad_(), u)
