@@ -262,16 +262,15 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
         n = block_sum64(n);
         u64 m = greedy ? 1 : by_k ? min(n, (u64)k_row) : n;
         if (by_p) m = max((u64)1, (u64)ceil((double)fmaxf(p_row, 0.0f) * (double)m));
-        if (wave == 0) {
-            const double u = a.u[row];
-            u64 j = !greedy && u > 0.0 ? (u64)fmin(u * (double)m, (double)m) : 0;
-            nth(min(j, m - 1) + 1, is);
-            if (lane == 0) {
-                a.id[row] = sh.found_id;
-                if (a.p) a.p[row] = (float)(1.0 / (double)m);
-                if (a.logprob) a.logprob[row] = (float)-log((double)n);
-                if (a.n_kept) a.n_kept[row] = (int)m;
-            }
+        const double u = a.u[row];
+        const u64 j = !greedy && u > 0.0 ? (u64)fmin(u * (double)m, (double)m) : 0;
+        if (wave == 0) nth(min(j, m - 1) + 1, is);
+        __syncthreads();                                                  // some lane has left found_id
+        if (tid == 0) {
+            a.id[row] = sh.found_id;
+            if (a.p) a.p[row] = (float)(1.0 / (double)m);
+            if (a.logprob) a.logprob[row] = (float)-log((double)n);
+            if (a.n_kept) a.n_kept[row] = (int)m;
         }
         return;
     }

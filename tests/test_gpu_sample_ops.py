@@ -272,3 +272,19 @@ def test_rows_whose_first_ids_are_masked(dt):
     x[:, :18500] = -math.inf
     u = torch.rand((8,), generator=g, dtype=torch.float64).tolist()
     check(x, u, t=[1.0] * 8, k=[0, 40, 0, 600, 1, 1499, 0, 5], p=[1.0, 1.0, 0.9, 1.0, 1.0, 0.95, 0.5, 0.7], m=[0.0] * 6 + [0.05] * 2)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_rows_of_infinities_wherever_the_drawn_one_lies(dt):
+    """The drawn infinity in every lane and element of a wave's load, in the first, a middle and the last group, alone and among others."""
+    v = 3000
+    at = torch.cat([torch.arange(0, 520), torch.arange(1400, 1500), torch.arange(v - 300, v)])
+    x = torch.zeros((len(at), v), dtype=dt)
+    x[torch.arange(len(at)), at] = math.inf
+    u = torch.rand(len(at), generator=torch.Generator().manual_seed(21), dtype=torch.float64).tolist()
+    r = check(x, u)
+    assert torch.equal(r.id.cpu().long(), at)
+    x[:, [7, 900, 2999]] = math.inf
+    check(x, u)
+    check(x, u, k=[2] * len(at))
+    check(x, u, t=[0.0] * len(at))
