@@ -63,7 +63,7 @@ template <typename T> struct Row {
 
 struct Weight {                    // w(x) 2^S in double and as an integer
     const double* table;           // LDS: 2^(j/1024 + S)
-    double top, c, least;          // y = (x - top) c; below `least` w 2^S is less than 2^-16 and counts as that, which rounds to 0
+    double top, c, least;          // y = (x - top) c; below `least` (-150 at least) w 2^S is less than 2^-16 and counts as that, which rounds to 0
     __device__ __forceinline__ double scaled(float x) const {
         const double y = fmax(((double)x - top) * c, least);
         constexpr double magic = 6755399441055744.0 / 1024.0;            // 1.5 2^52 / 1024: adding it rounds y to a multiple of 1/1024
@@ -73,7 +73,7 @@ struct Weight {                    // w(x) 2^S in double and as an integer
         constexpr double L1 = 0.693147180559945309417, L2 = 0.240226506959100712333;
         const double q = r * fma(r, L2, L1);
         const double t = table[k & 1023];
-        const double s = __hiloint2double(__double2hiint(t) + ((k >> 10) << 20), __double2loint(t));  // the exponent: -16 <= k / 1024 + S <= 51
+        const double s = __hiloint2double(__double2hiint(t) + ((k >> 10) << 20), __double2loint(t));  // the exponent: least + S <= k / 1024 + S <= 51
         return fma(s, q, s);
     }
     static __device__ __forceinline__ u64 integer(double s) {            // round(s), 0 <= s <= 2^51
@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     // an infinite or vanishing t must not meet a difference of 0 or infinity
     const double c = fmax(fmin(1.44269504088896340736 / (greedy ? 1.0 : (double)t_row), 1e300), 1e-300);
     const double one = ldexp(1.0, S);
-    const Weight wt{sh.table, (double)top, c, -(double)(S + 16)};
+    Weight wt{sh.table, (double)top, c, -(double)(S + 16)};
     const int k_row = a.top_k ? a.top_k[row] : 0;
     const float p_row = a.top_p ? a.top_p[row] : 1.0f;
     const bool by_k = !greedy && k_row > 0 && k_row < a.n_vocab, by_p = !greedy && p_row < 1.0f;
@@ -230,6 +230,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(ss_sample_rows_ar
     if (a.min_p && !(a.min_p[row] == a.min_p[row])) m_row = 0.0f;
     const bool by_m = !greedy && m_row > 0.0f;
     const double m_scaled = (double)m_row * one;
+    if (by_m) wt.least = fmin(wt.least, log2((double)m_row) - 1.0);      // weights around min_p have to be told apart, however small it is
 
     // the sum of all weights, for logprob: of float32 exponentials where some pass goes over the whole row and needs no exact ones, else exact
     float part = 0.0f;

@@ -288,3 +288,20 @@ def test_rows_of_infinities_wherever_the_drawn_one_lies(dt):
     check(x, u)
     check(x, u, k=[2] * len(at))
     check(x, u, t=[0.0] * len(at))
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("v", [900, 40000])
+def test_min_p_below_the_weights_steps(dt, v):
+    """min_p from 1e-14 to float32's smallest: ids too light to be drawn are still counted or left out as the rule says."""
+    g = torch.Generator().manual_seed(22)
+    m = [1e-14, 1e-16, 1e-18, 1e-20, 1e-25, 1e-38, 1e-44, 1e-30, 1e-22]
+    n = len(m)
+    x = torch.randn((n, v), generator=g) * 12
+    x[:, 11] = 40.0
+    x[-1, 5:200] = torch.finfo(dt).min
+    x = x.to(dt)
+    u = torch.rand(n, generator=g, dtype=torch.float64).tolist()
+    check(x, u, m=m)
+    check(x, u, t=[0.5] * n, m=m)
+    check(x, u, t=[0.7] * n, k=[50, 0, 700, 0, 880, 0, 3, 0, 0], p=[1.0, 0.9] * 4 + [1.0], m=m)
