@@ -106,7 +106,7 @@ class KvCache:
         _need(k.dtype in held and v.dtype == k.dtype, f"k and v must be {held[0]}, got {k.dtype} and {v.dtype}")
         _need(k.dim() == 4 and v.shape == k.shape, "k and v must be [n_pages, n_kv_heads, page_size, head_dim], alike")
         n, heads, page, dim = k.shape
-        _need(all(t.stride()[1:] == (page * dim, dim, 1) for t in (k, v)) and (n == 1 or k.stride(0) == v.stride(0)), "each page must be contiguous, k and v with one stride between pages")
+        _need(all(t.stride()[2:] == (dim, 1) and (heads == 1 or t.stride(1) == page * dim) for t in (k, v)) and (n == 1 or k.stride(0) == v.stride(0)), "each page must be contiguous, k and v with one stride between pages")
         scales = None
         if self.kind == KV_SAME:
             _need(k_scale is None and v_scale is None, "a 16-bit cache has no scales")
@@ -115,7 +115,7 @@ class KvCache:
             for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
                 _on(t, k.device, name)
                 _need(t.dtype == scales and t.shape == k.shape[:3], f"{name} must be {scales} [n_pages, n_kv_heads, page_size]")
-                _need(t.stride()[1:] == (page, 1) and (n == 1 or t.stride(0) == k_scale.stride(0)), "each page's scales must be contiguous, with one stride between pages")
+                _need(t.stride(2) == 1 and (heads == 1 or t.stride(1) == page) and (n == 1 or t.stride(0) == k_scale.stride(0)), "each page's scales must be contiguous, with one stride between pages")
         self.k, self.v, self.k_scale, self.v_scale, self.dtype, self.device, self.index = k, v, k_scale, v_scale, dtype, k.device, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = n, heads, page, dim
         self._real = [(t, name) for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)) if t is not None and t.is_floating_point()]

@@ -192,3 +192,21 @@ def test_append_of_infinities(kind, dt, dim):
                 assert math.isnan(g) if math.isnan(v) or (mixed and math.isinf(v)) else g == sign * v if math.isinf(v) else True, (t, i, v, g)
         if kind == "same":
             assert torch.equal(torch.nan_to_num(got, 7.0), torch.nan_to_num(sign * x, 7.0))
+
+
+@pytest.mark.parametrize("kind", ["same", "e4m3", "int8"])
+def test_a_cache_of_one_head_seen_the_other_way_round(kind):
+    """[page, row, head] tensors of one head are [page, head, row] ones: the stride over a single head says nothing."""
+    st = Step([40, 33], [40, 33], 1, 64, 16, kind, "f16")
+    plain, batch = st.cuda()
+    turn = lambda t: torch.empty_strided(t.shape, (t.stride(0), t.stride(2)) + t.stride()[2:], dtype=t.dtype, device="cuda").copy_(t)  # noqa: E731
+    turned = [None if t is None else turn(t) for t in (plain.k, plain.v, plain.k_scale, plain.v_scale)]
+    assert turned[0].stride(1) == 64 and (kind == "same" or turned[2].stride(1) == 1)
+    cache = ops.KvCache(*turned, kind=kind, dtype=st.dt)
+    x = [st.rows((st.n, 1, 64)).cuda() for _ in "kvq"]
+    for c in (plain, cache):
+        ops.kv_append(c, batch, x[0], x[1])
+    assert all(torch.equal(a, b) for a, b in zip(ops.kv_read(plain, batch), ops.kv_read(cache, batch)))
+    assert torch.equal(ops.kv_attention(plain, batch, x[2]), ops.kv_attention(cache, batch, x[2]))
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.KvCache(torch.zeros((4, 16, 2, 64), dtype=torch.float16, device="cuda").transpose(1, 2), torch.zeros((4, 2, 16, 64), dtype=torch.float16, device="cuda"))
