@@ -1,5 +1,5 @@
 // Dev tool: run launch_enc_attention on seeded random q/k/vT for several (B, H, Tn) and write the outputs; compare two runs made with
-// different SS_ATTN_LDS settings.  hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/attn_test.cpp speaksense_amd/csrc/kernels_attn.hip -Ispeaksense_amd/csrc
+// different SS_ATTN_LDS settings.  hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/attn_test.cpp speaksense_amd/csrc/kernels_attn.hip -Ispeaksense_amd/csrc
 #include <cstdio>
 #include <cstdlib>
 #include <vector>

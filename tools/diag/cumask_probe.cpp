@@ -1,6 +1,6 @@
 // Which XCDs / CUs does a stream created with hipExtStreamCreateWithCUMask run on, for a given bit pattern -- launched directly and replayed
 // from a captured hipGraph?  (dev tool, run on the GPU box: lanes confined to disjoint CU sets)
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/diag/cumask_probe.cpp -o /tmp/cumask_probe && /tmp/cumask_probe
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/diag/cumask_probe.cpp -o /tmp/cumask_probe && /tmp/cumask_probe
 // Every workgroup records HW_REG_XCC_ID and HW_REG_HW_ID (CU / SE fields) and spins ~20 us so that the launch spreads over all CUs it may use.
 #include <hip/hip_runtime.h>
 #include <cstdio>

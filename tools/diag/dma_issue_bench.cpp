@@ -1,7 +1,7 @@
 // What does one LDS-DMA instruction (global_load_lds_dwordx4, 1 KB per wave) cost the issuing wave, as a function of how its 64 lanes' 16-byte
 // pieces are laid out in global memory?  (dev tool, run on the GPU box; DESIGN.md section 8a: the staging waves' DMA issue is the critical path of
 // the 256 x 256 GEMM's main loop)
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/diag/dma_issue_bench.cpp -o tools/diag/dma_issue_bench.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/diag/dma_issue_bench.cpp -o tools/diag/dma_issue_bench.bin
 // Shapes: lanes-per-row L in {4, 8, 16, 64}: a wave instruction touches 64 / L rows of 16 L contiguous bytes each (row pitch 2560 B = a K = 1280
 // f16 operand).  L = 4 is what gemm256_kernel issues (TK = 32: 64-byte rows), L = 8 a TK = 64 layout, L = 64 one contiguous kilobyte.
 // Reported: shader cycles per instruction between the first and the last issue of a burst of 32 (s_memtime), 1 / 2 / 4 / 8 waves per workgroup

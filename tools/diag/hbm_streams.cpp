@@ -1,5 +1,5 @@
 // How much HBM bandwidth do S CONCURRENT decoder cross-attention launches get in total?  (dev tool, run on the GPU box)
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/diag/hbm_streams.cpp speaksense_amd/csrc/kernels_decode.hip -Ispeaksense_amd/csrc -o /tmp/hbm_streams
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/diag/hbm_streams.cpp speaksense_amd/csrc/kernels_decode.hip -Ispeaksense_amd/csrc -o /tmp/hbm_streams
 // Each stream owns a cross-KV region of 32 windows x (K, V) x 20 heads x 1500 x 64 f16 (246 MB: one large-v3 layer for a 32-row pass) and
 // launches the unsplit kernel `reps` times back to back; wall time over all streams -> aggregate GB/s.
 #include <chrono>

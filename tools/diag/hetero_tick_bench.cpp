@@ -1,5 +1,5 @@
 // Premise check for a "heterogeneous tick" decoder pass (dev tool, run on the GPU box; DESIGN.md section 8a, "what next"):
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/diag/hetero_tick_bench.cpp -o tools/diag/hetero_tick_bench.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/diag/hetero_tick_bench.cpp -o tools/diag/hetero_tick_bench.bin
 // A decoder pass is a chain of ~10 latency-bound launches per layer plus one HBM-streaming cross-attention launch; lanes overlap the two kinds
 // across independent row groups, but each kernel doubles in duration under the other lanes' traffic.  The alternative this tool
 // prices: ONE launch per chain step that carries the chain kernel of row group B AND a tenth of the cross-attention key range of row group A (whose

@@ -1,5 +1,5 @@
 // Dev tool (round 6): how fast can ONE CU get a 256 x 256 output tile out to memory, by request shape, row pitch, cache policy and number of CUs storing?
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/diag/store_rate_bench.cpp -o tools/diag/store_rate_bench.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 tools/diag/store_rate_bench.cpp -o tools/diag/store_rate_bench.bin
 // The GEMM epilogues (kernels_gemm.hip epilogue256) move a 128 KB (f16) / 256 + 256 KB (f32 residual) tile per CU at 12 - 14 B/clk whatever was tried there
 // (deeper operand prefetch, a start stagger: tools/experiments/r06_gemm_stagger/).  This isolates the store path: one 512-thread workgroup per CU (96 KB of dynamic
 // LDS keeps a second one off the CU), every workgroup writes TILES tiles of 256 rows x 512 bytes into a matrix of row pitch `pitch`, s_memtime around the stores

@@ -1,6 +1,6 @@
 # gpurun -- 'bash tools/gpu_r05_l.sh': gemm256k64 main loop with the two waves of a SIMD issuing their LDS-DMA in different quarters (-DSS_K64_DMA_STAGGER), A / B / A / B
 cd "$GRAFT_REPO_ROOT" && mkdir -p gpurun_out
-B="hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/gemm_bench.cpp speaksense_amd/csrc/kernels_gemm.hip -Ispeaksense_amd/csrc"
+B="hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/gemm_bench.cpp speaksense_amd/csrc/kernels_gemm.hip -Ispeaksense_amd/csrc"
 $B -o /tmp/gb_base 2>/dev/null || exit 1
 $B -DSS_K64_DMA_STAGGER -o /tmp/gb_stag 2>/dev/null || exit 1
 OUT=gpurun_out/r05_l_gemm_dma_stagger_ab.txt

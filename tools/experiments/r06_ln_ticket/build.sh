@@ -4,7 +4,7 @@ cd /root/repo
 python -c "from speaksense_amd import build; build.build()"
 mkdir -p gpurun_ab
 for src in kernels_decode.hip engine.cpp; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -x hip -DSS_EXP_LN_TICKET -Ispeaksense_amd/csrc -c speaksense_amd/csrc/$src -o gpurun_ab/exp_$src.o &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -fPIC -Wno-unused-function -x hip -DSS_EXP_LN_TICKET -Ispeaksense_amd/csrc -c speaksense_amd/csrc/$src -o gpurun_ab/exp_$src.o &
 done
 wait
 objs=""

@@ -1,5 +1,5 @@
 // Standalone GEMM micro-benchmark / correctness harness for kernels_gemm.hip (dev tool, run on the GPU box):
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/gemm_bench.cpp speaksense_amd/csrc/kernels_gemm.hip -Ispeaksense_amd/csrc -o /tmp/gemm_bench
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/gemm_bench.cpp speaksense_amd/csrc/kernels_gemm.hip -Ispeaksense_amd/csrc -o /tmp/gemm_bench
 #include <algorithm>
 #include <cmath>
 #include <cstdio>

@@ -1,5 +1,5 @@
 // Decode GEMV micro-benchmark (dev tool): time dec_gemv_kernel for the large-v3 decode shapes over (S, NW) plans.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -x hip tools/gemv_bench.cpp speaksense_amd/csrc/kernels_decode.hip -Ispeaksense_amd/csrc -o tools/gemv_bench.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -x hip tools/gemv_bench.cpp speaksense_amd/csrc/kernels_decode.hip -Ispeaksense_amd/csrc -o tools/gemv_bench.bin
 #include <cstdio>
 #include <cstdlib>
 #include <vector>

@@ -1,5 +1,5 @@
 // Dev tool: cost of a software grid barrier vs a kernel boundary on MI355X, and of barrier-separated weight-streaming phases.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/gridsync_bench.cpp -o tools/gridsync_bench.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 tools/gridsync_bench.cpp -o tools/gridsync_bench.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,7 +1,7 @@
 // Dev tool ("measure the flag path first with a 2-kernel microbenchmark"): what does one DEPENDENT hand-off between two groups of
 // workgroups cost on MI355X -- as a kernel boundary inside a captured hipGraph (what the decoder pass uses today) and as a flag hand-off inside one
 // persistent kernel (what a fused per-block kernel would use)?
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/handoff_bench.cpp -o tools/handoff_bench.bin
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 tools/handoff_bench.cpp -o tools/handoff_bench.bin
 // Two groups A and B of G workgroups (256 threads) ping-pong: every workgroup of a group writes a 4 KB payload; a workgroup of the other group may
 // start its turn when (p2p) ITS partner's payload or (all) EVERY payload of the previous turn is visible, reads 4 KB of it, and writes its own.
 // One turn = one hand-off; the decoder pass is a chain of ~350 of them (split-K GEMV -> reduce + LayerNorm -> GEMV -> attention -> ...), all of the

@@ -1,4 +1,4 @@
-// Dev tool: every helper of wave_ops.h against the __shfl_xor butterfly it replaces.  hipcc --offload-arch=gfx950 -O3 -Ispeaksense_amd/csrc tools/waveops_test.cpp
+// Dev tool: every helper of wave_ops.h against the __shfl_xor butterfly it replaces.  hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -Ispeaksense_amd/csrc tools/waveops_test.cpp
 #include <cstdio>
 #include <vector>
 #include "wave_ops.h"
