@@ -272,8 +272,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, int shift, T* __
 // m_q need not be the maximum, only near it: it moves when a score exceeds it by more than 2^8 (p then is at most 2^8, in f16 as in bf16), which
 // leaves most tiles without a reduction across lanes and without rescaling O.
 //
-// At the bottom f16 holds a term p v_j / sref in full only from 2^-14 on, and sref may belong to a key that a row does not see or that weighs nothing there.  So
-// over 8-bit caches all p of a row are taken 2^lift higher (l, O and p alike: the division takes it out): 2^5, and where the row's largest term lies
+// At the bottom f16 holds a number in full only from 2^-14 on.  So over f16 caches all p of a row are taken 2^7 higher (l, O and p alike: the division takes it
+// out; p is at most 2^(8 + 7)): a long tail of probabilities down to 2^-21 of the largest keeps its digits.  Over 8-bit caches f16 holds p v_j / sref, and sref may
+// belong to a key that a row does not see or that weighs nothing there: all p of a row are taken 2^lift higher, 2^5, and where the row's largest term lies
 // below 2^-8, as much more as brings it to 1, as far as float32 holds p (2^121; l is kept 2^64 lower, so that its sum stays in range too).  Terms then reach
 // 2^(8 + 2 + 5) at most, and the row's largest lies at 2^-3 or above.  It is looked for only where m or sref moved and while some row of the wave is low; in
 // between it can only grow.
@@ -293,7 +294,8 @@ struct AttnArgs {
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kSlack = 8.0f;         // log2 of the largest probability relative to m
 constexpr float kRefRange = 4.0f;      // of a value's scale above sref
-constexpr float kLift = 5.0f, kLow = -8.0f, kMostLift = 121.0f;     // 8-bit caches, in log2 units
+template <typename M, bool SCALED> constexpr float kLift = std::is_same<M, bf16>::value ? 0.0f : SCALED ? 5.0f : 7.0f;      // in log2 units
+constexpr float kLow = -8.0f, kMostLift = 121.0f;     // 8-bit caches
 constexpr float kDown = 0x1p-64f;      // 8-bit caches: on l
 
 template <int KIND> struct Held;       // what the MFMA multiplies, and bytes of an element
@@ -414,13 +416,13 @@ template <typename M, bool SCALED, int D> struct Row {
     }
     __device__ __forceinline__ float m(float c) const { return raw * c; }        // in log2 units
     __device__ __forceinline__ float lift() const {          // a whole number; l and o hold 2^lift times the sums relative to 2^m
-        return !SCALED ? 0.0f : big < kLow && big > -kInf ? kLift + fminf(ceilf(-big), kMostLift) : kLift;
+        return kLift<M, SCALED> + (SCALED && big < kLow && big > -kInf ? fminf(ceilf(-big), kMostLift) : 0.0f);
     }
     __device__ __forceinline__ float unlift() const { return __uint_as_float((unsigned)(127 - (int)lift()) << 23); }
     __device__ __forceinline__ void sum(float w) { l = SCALED ? fmaf(w, kDown, l) : l + w; }
     __device__ __forceinline__ float total() const {          // relative to 2^m
         const float t = rows_sum(l);
-        return SCALED ? t * unlift() * (1.0f / kDown) : t;
+        return t * unlift() * (SCALED ? 1.0f / kDown : 1.0f);
     }
     __device__ __forceinline__ void scale(float a) {
         l *= a;
@@ -450,7 +452,7 @@ __device__ __forceinline__ void softmax_ref(Row<M, SCALED, D>* st, Gauge& ga, fl
         for (int e = 1; e < NE; e++) top[j] = fmaxf(top[j], x[j][e]);
         const float m = st[j].m(c[j]);
         moved |= top[j] * c[j] > m + kSlack;
-        ref[j] = (m == -kInf ? 0.0f : m) - (SCALED ? kLift : 0.0f);
+        ref[j] = (m == -kInf ? 0.0f : m) - kLift<M, SCALED>;
     }
     if (__ballot(moved) || ga.far || ga.low) {
         asm volatile("");              // a branch, not selects
@@ -491,7 +493,9 @@ __device__ __forceinline__ void softmax_ref(Row<M, SCALED, D>* st, Gauge& ga, fl
                 ref[j] -= lift;
             }
             ga.low = __ballot(w) != 0;
-        }
+        } else
+#pragma unroll
+            for (int j = 0; j < QC; j++) ref[j] -= kLift<M, SCALED>;
     }
 }
 // 8 scores of a lane -> its B operand

@@ -210,3 +210,32 @@ def test_a_cache_of_one_head_seen_the_other_way_round(kind):
     assert torch.equal(ops.kv_attention(plain, batch, x[2]), ops.kv_attention(cache, batch, x[2]))
     with pytest.raises(ValueError, match="contiguous"):
         ops.KvCache(torch.zeros((4, 16, 2, 64), dtype=torch.float16, device="cuda").transpose(1, 2), torch.zeros((4, 2, 16, 64), dtype=torch.float16, device="cuda"))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["same", "e4m3", "int8"])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("n,log2,cut", [(60000, 20, True), (4000, 20, False), (300, 18, False)])
+def test_a_long_tail_below_one_key(dt, kind, new, n, log2, cut):
+    """One key takes nearly all weight and holds a value of zero: what comes out is the sum of the tail, whose probabilities all are alike, so that a rounding of
+    theirs would show in full (cut False: one workgroup takes all keys, as in a call of many sequences).  Bound: as above, with the tail's own terms normal f16 numbers (2^7 2^-20 > 2^-14; 8-bit caches: lifted to the row's largest)."""
+    st = Step([n], [new], 1, 64, 256, kind, dt)
+    k = torch.zeros(st.k.shape)
+    v = torch.ones(st.k.shape)
+    pg, r = int(st.table[0, 3 // 256]), 3
+    k[pg, 0, r, 0] = (log2 - math.log2(1.03)) * math.log(2.0) * 8 / 4
+    v[pg, 0, r] = 0
+    refill(st, k, v)
+    q = torch.zeros((st.n, 3, 64), dtype=st.dt)
+    q[..., 0] = 4.0
+    st.cuda()
+    x = float(st.dense(0, "k")[3, 0, 0]) * 4 / 8          # the cached key's score
+    one = float(st.dense(0, "v")[0, 0, 0])
+    seen = torch.arange(n - new, n, dtype=torch.float64) if new > 1 else torch.tensor([n - 1.0], dtype=torch.float64)
+    p = math.exp(-x)
+    want = (seen * p * one / (1 + seen * p))[:, None, None]
+    half_out, half_p = torch.finfo(st.dt).eps / 2, torch.finfo(torch.bfloat16 if kind == "same" and dt == "bf16" else torch.float16).eps / 2
+    batch = ops.KvBatch(st.batch.page_table, st.batch.q_start, st.batch.kv_len, n_tokens=st.n, max_new=new, max_len=n if cut else 1)
+    assert (ops._lib().ss_kv_attention_workspace(st.cache._c, batch._c, 3) > 0) == cut
+    got = ops.kv_attention(st.cache, batch, q.cuda()).cpu().double()
+    assert ((got - want).abs() <= (half_out + half_p + 2.0 ** -15 + 2.0 ** -20) * want).all(), float(((got - want) / want).abs().max())
