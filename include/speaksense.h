@@ -419,7 +419,8 @@ int ss_kv_read(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss_kv_r
 /* softmax(scale q K^T) V of the new tokens' queries [n_tokens][n_heads][head_dim] over their sequence's keys, which ss_kv_append has written, the new
  * ones among them.  Query head i reads key head i / (n_heads / n_kv_heads).  causal != 0: a token sees the positions up to its own; 0: all kv_len of
  * them (cross-attention).  Keys on no page are not seen.  A token that sees no key gets zeros (lse -inf).  Rows of pages behind kv_len may hold anything; keys
- * and values that some token of the sequence sees are taken to be finite.
+ * and values that some token of the sequence sees are taken to be finite, and so are the sums of probability * value before they are divided (float32, the
+ * probabilities up to 2^15).  A query that holds a NaN or an infinity gives NaN, to its own token and head only.
  * out: as q, not overlapping it or the cache.  lse (optional): float32 [n_tokens][n_heads], the natural logarithm of the softmax's denominator, with which results over disjoint keys
  * are joined.  Softmax and sums are held in float32; the probabilities are rounded to the type that the matrix product takes (dtype; f16 for 8-bit
  * caches, whose codes it holds exactly).  In an 8-bit cache each token's terms probability * scale are rounded relative to the largest that this token sees, so

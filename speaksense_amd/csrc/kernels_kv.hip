@@ -716,7 +716,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
     M4 = fmaxf(fmaxf(s_m[0][oc], s_m[1][oc]), fmaxf(s_m[2][oc], s_m[3][oc]));
     float L = 0.0f, acc[N];
 #pragma unroll
-    for (int w = 0; w < 4; w++) L += M4 == -kInf ? 0.0f : s_l[w][oc] * __builtin_amdgcn_exp2f(s_m[w][oc] - M4);
+    for (int w = 0; w < 4; w++) L += s_l[w][oc] * (M4 == -kInf ? 1.0f : __builtin_amdgcn_exp2f(s_m[w][oc] - M4));      // m -inf: no key (l = 0), or a query of NaN (l = NaN)
 #pragma unroll
     for (int k = 0; k < N; k++) acc[k] = (s_o[0][oc][col + k] + s_o[1][oc][col + k]) + (s_o[2][oc][col + k] + s_o[3][oc][col + k]);
     const int orow = sp.q0 + oc / t.G, ohead = h * t.G + oc % t.G;

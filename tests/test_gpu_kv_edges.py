@@ -239,3 +239,21 @@ def test_a_long_tail_below_one_key(dt, kind, new, n, log2, cut):
     assert (ops._lib().ss_kv_attention_workspace(st.cache._c, batch._c, 3) > 0) == cut
     got = ops.kv_attention(st.cache, batch, q.cuda()).cpu().double()
     assert ((got - want).abs() <= (half_out + half_p + 2.0 ** -15 + 2.0 ** -20) * want).all(), float(((got - want) / want).abs().max())
+
+
+@pytest.mark.parametrize("kind", ["same", "e4m3", "int8"])
+@pytest.mark.parametrize("new,groups", [(1, 8), (40, 2)])
+def test_queries_of_nan_and_infinity_keep_to_themselves(kind, new, groups):
+    """Rows of the same tile, wave and workgroup stay within their bounds beside rows that can only be NaN."""
+    st = Step([700, 90, 64], [new] * 3, 1, 64, 16, kind, "bf16")
+    q = (torch.randn((st.n, groups, 64), generator=st.g) * 1.5).to(st.dt)
+    st.cuda()
+    want, tol = attend_seen(st, q, 0.125, True)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool)
+    for t, h, v in ((0, 1, math.nan), (new - 1, 0, math.inf), (st.n - 1, 1, -math.inf)):
+        q[t, h, 5] = v
+        bad[t, h] = True
+    for max_len in (1, 700):
+        b = ops.KvBatch(st.batch.page_table, st.batch.q_start, st.batch.kv_len, n_tokens=st.n, max_new=new, max_len=max_len)
+        got = ops.kv_attention(st.cache, b, q.cuda()).cpu().double()
+        assert ((got - want).abs() <= tol)[~bad].all() and torch.isnan(got[bad]).all()
