@@ -17,6 +17,7 @@ from . import binding
 
 KV_SAME, KV_E4M3, KV_INT8 = 0, 1, 2
 _KINDS = {"same": KV_SAME, "e4m3": KV_E4M3, "int8": KV_INT8, KV_SAME: KV_SAME, KV_E4M3: KV_E4M3, KV_INT8: KV_INT8}
+_DUAL = forward_ad if hasattr(forward_ad, "_current_level") else NamedTuple("Always", [("_current_level", int)])(0)      # a level below 0: no duals anywhere
 _DTYPES = {torch.bfloat16: binding.DTYPE_BF16, torch.float16: binding.DTYPE_F16, torch.float32: 3}
 
 
@@ -77,7 +78,7 @@ def _on(t, device, name):
 def _no_gradient(t, name):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not have")
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    if _DUAL._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} carries a forward-mode gradient, which this operator does not have")
 
 
@@ -164,7 +165,7 @@ class KvBatch:
 def _rows(t, name, cache, batch, heads):
     """The C view of token rows [n_tokens, heads, head_dim]; `heads` None: any number."""
     if isinstance(t, torch.Tensor) and t.dtype is cache.dtype and t.get_device() == cache.index:
-        if t.requires_grad or forward_ad._current_level >= 0:
+        if t.requires_grad or _DUAL._current_level >= 0:
             _no_gradient(t, name)
         shape = t.shape
         if len(shape) == 3 and shape[0] == batch.n_tokens and shape[2] == cache.head_dim and (heads is None or shape[1] == heads):
@@ -182,7 +183,7 @@ def _same_device(cache, batch):
     _need(isinstance(cache, KvCache) and isinstance(batch, KvBatch), "expected a KvCache and a KvBatch")
     _need(batch.index == cache.index, "the batch and the cache are on different devices")
     for t, name in cache._real:
-        if t.requires_grad or forward_ad._current_level >= 0:
+        if t.requires_grad or _DUAL._current_level >= 0:
             _no_gradient(t, name)
 
 
@@ -250,7 +251,7 @@ def sample_rows(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=No
         if not (isinstance(t, torch.Tensor) and t.get_device() == index and t.dtype is dt and t.shape == (n,) and t.is_contiguous()):
             _on(t, dev, name)
             raise ValueError(f"{name} must be {dt} [{n}], contiguous")
-        if t.requires_grad or forward_ad._current_level >= 0:
+        if t.requires_grad or _DUAL._current_level >= 0:
             _no_gradient(t, name)
         ptr.append(t.data_ptr())
     whole, real = torch.empty((2, n), dtype=torch.int32, device=dev), torch.empty((2, n), dtype=torch.float32, device=dev)
