@@ -435,7 +435,8 @@ int ss_kv_attention(const ss_kv_cache* cache, const ss_kv_batch* batch, const ss
  * weight (ties: of id), have less than top_p of what top_k left; min_p keeps ids with w_i >= min_p.  The best id is always kept.  Drawn is the first kept id, in
  * order of id, whose running sum of kept weights exceeds u times their total: std::discrete_distribution's rule for a given uniform number.
  * Weights are held as integers of 2^-bits of the largest (bits = 62 - log2 of the vocabulary, rounded down, 51 at most), so sums are exact and
- * do not depend on the order; a draw can differ from the real numbers' only where u falls within about 1e-12 of a boundary.
+ * do not depend on the order.  Each is off by 1e-11 of itself and half such an integer at most, so a draw or a cut by top_p can differ from the real numbers' only
+ * where it falls within 1e-11 + n_vocab 2^-(bits + 1) of a boundary: 4e-10 for 51866 ids, 1.2e-11 for 4096, 1.2e-7 for 2^20.
  * Settings per row may be NULL (off; temperature 1) and need no host value: t <= 0 or NaN takes the best id, top_k <= 0 or >= n_vocab, top_p >= 1 or NaN, min_p <= 0
  * or NaN switch a filter off; min_p > 1 counts as 1; u is taken into [0, 1).  A row without any unmasked id gives id -1, p 0, logprob -inf, n_kept 0. */
 typedef struct ss_sample_rows_args {
@@ -447,7 +448,8 @@ typedef struct ss_sample_rows_args {
     const float* min_p;
     int32_t* id;                  /* [n_rows] results */
     float* p;                     /* weight of the id among the kept ones (1 where t <= 0); may be NULL */
-    float* logprob;               /* ln of its probability before the filters, at temperature t (1 where t <= 0); may be NULL */
+    float* logprob;               /* ln of its probability before the filters, at temperature t (1 where t <= 0); may be NULL.  Its denominator is a float32
+                                     sum where top_k or t <= 0 is set, or min_p without top_p, good to about 2^-20; else that of the integers */
     int32_t* n_kept;              /* ids left by the filters (1 where t <= 0); may be NULL */
     int64_t row_stride;           /* elements, >= n_vocab */
     int32_t n_rows;               /* <= 2^21 */

@@ -31,8 +31,8 @@ __device__ __forceinline__ float gelu_tanh_f(float x) {
 }
 // The same GELU for the four accumulator values a lane owns, two at a time with the constants folded: per element 1 add (bias, done by the caller) +
 // 3 mul + 1 fma + 1 add, 1 v_exp_f32 + 1 v_rcp_f32, and -- ROUND_IN, ggml's f16 GELU table input -- half a v_cvt_pk_f16_f32 (RNE) + one v_cvt_f32_f16.
-// (The build forbids packed-f32 instructions, build.py; with them the large-v3 benchmark ran no faster: 3201 / 3257 against 3307 / 3282 xRT, two runs
-// of each in turn.)  exp(-2u) = 2^(x * (C1 + C3 x^2)), C1 = -2 sqrt(2/pi) log2(e), C3 = 0.044715 C1.
+// (The build forbids packed-f32 instructions, build.py.  Two runs of the large-v3 benchmark each, in turn: 3201 / 3257 xRT with them, 3307 / 3282 without; runs on
+// different days differ by as much.)  exp(-2u) = 2^(x * (C1 + C3 x^2)), C1 = -2 sqrt(2/pi) log2(e), C3 = 0.044715 C1.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 template <bool ROUND_IN>

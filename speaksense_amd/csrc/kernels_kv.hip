@@ -543,7 +543,7 @@ template <typename T, int N> __device__ __forceinline__ void store_cols(T* p, co
 // ---- few query rows (max_new G <= 16): grid (sequences x splits, key heads); the 4 waves of a workgroup take every fourth 32-key tile of its key
 // range straight from memory into registers (the next tile's loads fly while one is computed) and merge at the end.  HBM-bound: with G <= 16 the
 // MFMA issues of a tile take ~1/10 of the time its bytes need at the card's rate, so the 15 idle columns of a one-head row cost nothing.
-// 4 contexts of 30001..65536 bf16 keys, 8 x 4 heads of 128: 116 us, 6.7 TB/s; 96 x 1500 e4m3 keys, 20 heads of 64: 76 us, 4.9 TB/s; a step of 8 short contexts: 9 us. ----
+// 4 contexts of 30001..65536 bf16 keys, 8 x 4 heads of 128: 116 us, 6.7 TB/s; 96 x 1500 e4m3 keys, 20 heads of 64: 76 us, 4.9 TB/s (74 without the rows' largest terms); a step of 8 short contexts: 9 us. ----
 template <int KIND, int D> struct KvTile {
     static constexpr int B = Held<KIND>::B, KN = D * B / 64;   // 16-byte pieces of a key row per lane
     u32x4 k[2][KN];
@@ -740,8 +740,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void kv_attn_few_kernel(KvArg
 // after that are on their way too; one barrier a tile.  V fragments come out of LDS by the transposing read (ds_read_b64_tr_b16: of each 16 lanes, lane i
 // names 4 columns of row i / 4 and receives 4 rows of column i), columns 16 n + (lane & 15) for MFMA n.
 // Bound by LDS (a 64-key tile is read once per wave: 106..117 B/clk for the keys, 57 for the transposing reads) and by the dependency chain of its two waves a
-// SIMD: 2 chunks of 2048 x 32 query heads over 16384 int8 keys of 128: 1.24 ms, 785 TFLOP/s, 65 % of what a large bf16 product reaches here; 16-bit keys 73 %.
-// Without its LDS reads it takes 740 us, without the exponentials 11 % less, without the staging 22 % less (16 bit 6 %). ----
+// SIMD: 2 chunks of 2048 x 32 query heads over 16384 int8 keys of 128: 1.21 ms, 806 TFLOP/s, 68 % of what a large bf16 product reaches here; 16-bit keys 73 %.
+// Without its LDS reads it took 740 us, without the exponentials 11 % less, without the staging 22 % less (16 bit 6 %); the rows' largest terms cost 1.5 %. ----
 template <typename M> __device__ __forceinline__ typename Mfma<M>::V8 read_tr(const char* p0, const char* p1) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds4;
@@ -750,7 +750,8 @@ template <typename M> __device__ __forceinline__ typename Mfma<M>::V8 read_tr(co
 }
 
 template <typename T, int KIND, int D, int QC>
-// (launch bounds: head_dim 64 with two column tiles at 3 waves a SIMD, 168 registers of the 172 that it would take)
+// (launch bounds: head_dim 64 with two column tiles at 3 waves a SIMD, 168 registers of the 172 that it would take: bf16 prompts over int8 45 us instead of 51.
+// With four, 256 registers hold all but 1 to 6 values over 8-bit caches, which spill: bf16 over int8 219 us where f16 takes 206)
 __global__ __launch_bounds__(256, D == 64 && QC == 2 ? 3 : 2) void kv_attn_tile_kernel(KvArgs a, AttnArgs t) {
     typedef typename Held<KIND>::M M;
     typedef typename Mfma<M>::V8 V8;
@@ -1142,8 +1143,9 @@ KvPlan kv_attention_plan(const ss_kv_cache& c, const ss_kv_batch& b, int n_heads
     // the spans of up to 16 rows, with a join of its own, was slower wherever both apply: 32 spans of 1..20 rows over 448 keys 27 us against 17, over 16384 keys
     // 689 against 460
     p.tile = rows > 16;
-    // Column tiles a wave.  4 read K and V out of LDS half as often, if they leave two workgroups a CU (head_dim 64, int8: 8 x 512 x 4 rows 208 us against 256,
-    // but 8 x 256 x 4 rows, one workgroup a CU, 176 against 134); at head_dim 128 they do not fit the registers
+    // Column tiles a wave.  4 read K and V out of LDS half as often, if they leave two workgroups a CU (head_dim 64, int8 codes and f16 tokens over 4096 keys:
+    // 8 x 512 x 4 rows 206 us against 241, but 8 x 256 x 4 rows, one workgroup a CU, 173 against 137; over 512 keys 40 against 36.5 and 27 against 24); at head_dim
+    // 128 they do not fit the registers
     const long wide = pairs * up(rows, 256);
     p.qc = rows <= 64 ? 1 : c.head_dim == 64 && rows >= 1024 && wide >= 512 ? 4 : 2;
     // As many key ranges as give the card 512 workgroups, none shorter than 512 keys (256 wanted: 1 x 128 x 4 rows over 16384 keys 87 us instead of 72; 1024 wanted:

@@ -11,8 +11,8 @@
 // equal; equal ids are then taken in the order of their number.
 //
 // Passes over the row, which stays in L2 after the first: the largest logit; k up to 512: one more for the ids above a bound; other k and top_p: the histogram and
-// the step's ids; a row that a list does not hold: the kept weights.  Bound by the vector instructions of those passes (the double exponential and the LDS
-// atomic of an id are some 40 of them), for few rows by the chain of barriers: 51866 float32 logits, 1 row 21 us, 160 rows without a filter 26, with k = 40 26, with
+// the step's ids; a row that a list does not hold: the kept weights.  Bound by the vector instructions of those passes on the one CU that a row has (the double
+// exponential and the LDS atomic of an id are some 40 of them: about 13 of the 21 us of a row of 51866), then by its chain of barriers: 51866 float32 logits, 1 row 21 us, 160 rows without a filter 26, with k = 40 26, with
 // top_p 0.9 at t = 1 58 (mixed settings 54: 620 GB/s), 512 rows of 128000 bfloat16 85 without a filter (1.5 TB/s), mixed 145.
 #include <algorithm>
 #include <type_traits>
@@ -623,7 +623,8 @@ void launch_sample_rows(const ss_sample_rows_args& a, hipStream_t st) {
     auto go = [&](auto t) {
         typedef decltype(t) T;
         const int groups = (a.n_vocab + Row<T>::GROUP - 1) / Row<T>::GROUP;
-        constexpr int most = (1 << 20) / Row<T>::GROUP * 8;               // beside ~51 KB of static LDS
+        constexpr int most = (1 << 20) / Row<T>::GROUP * 8;
+        static_assert(sizeof(Shared) + most <= 160 * 1024, "LDS of a workgroup: 57,648 bytes and 8 a group");
         static std::atomic<uint64_t> once{0};
         once_per_device(once, [&] { SS_HIP(hipFuncSetAttribute((const void*)sample_rows_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, most)); });
         sample_rows_kernel<T><<<a.n_rows, kThreads, (size_t)groups * 8, st>>>(a, S);
