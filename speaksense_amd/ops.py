@@ -142,7 +142,7 @@ class KvCache:
 
 class KvBatch:
     """The sequences of one step: page_table [n_seqs, max_pages], q_start [n_seqs + 1], kv_len [n_seqs] (int32, in device memory), and what the scheduler
-    knows on the host: the token rows n_tokens, the longest span of new tokens max_new, and optionally the shortest and the longest kv_len.
+    knows on the host: the token rows n_tokens, the longest span of new tokens max_new (kv_attention computes no more of a span), and optionally the shortest and the longest kv_len.
     The tensors may change between calls (a captured graph reads their contents at replay), the host's numbers belong to the object."""
 
     def __init__(self, page_table, q_start, kv_len, *, n_tokens, max_new, min_new=0, max_len=0):

@@ -257,3 +257,30 @@ def test_queries_of_nan_and_infinity_keep_to_themselves(kind, new, groups):
         b = ops.KvBatch(st.batch.page_table, st.batch.q_start, st.batch.kv_len, n_tokens=st.n, max_new=new, max_len=max_len)
         got = ops.kv_attention(st.cache, b, q.cuda()).cpu().double()
         assert ((got - want).abs() <= tol)[~bad].all() and torch.isnan(got[bad]).all()
+
+
+@pytest.mark.parametrize("kind", ["same", "e4m3", "int8"])
+@pytest.mark.parametrize("new,lens", SHAPES)
+def test_scores_beyond_2_to_the_12(kind, new, lens):
+    """Scores of thousands in log2 units that differ by halves, of exact products, over value rows of very different sizes; in each sequence they rise once from some
+    hundreds to thousands, so that the difference is formed first from there on."""
+    st = Step(lens, [new] * len(lens), 1, 64, 16, kind, "bf16")
+    top = {"same": 127.0, "e4m3": 448.0, "int8": 127.0}[kind]          # scale 1: the cache holds these keys exactly
+    k = torch.zeros(st.k.shape)
+    k[..., 2] = top
+    k[..., 1] = torch.randint(0, 11, k.shape[:3], generator=st.g).float()
+    v = torch.randn(k.shape, generator=st.g) * torch.exp2(torch.randint(-20, 21, k.shape[:3] + (1,), generator=st.g).float())
+    for s, n in enumerate(lens):
+        for p in range(n):
+            k[int(st.table[s, p // 16]), 0, p % 16, 0] = 8.0 if p < n // 2 else 120.0
+    refill(st, k, v)
+    q = torch.zeros((st.n, 3, 64), dtype=st.dt)
+    q[..., 0], q[..., 1] = 80.0, 1.0                      # 80 x 120 / 2 = 4800 in log2 units
+    q[:, 1] = -q[:, 1]
+    q[:, 2, 0] = 1.0
+    st.cuda()
+    scale = 0.5 * math.log(2.0)
+    for causal in (True, False):
+        want, tol = attend_seen(st, q, scale, causal)
+        got = ops.kv_attention(st.cache, st.batch, q.cuda(), scale=scale, causal=causal).cpu().double()
+        assert not torch.isnan(got).any() and ((got - want).abs() <= tol).all(), float(((got - want).abs() - tol).max())
